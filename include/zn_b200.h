@@ -168,6 +168,97 @@ ZN_API zn_status zn_loss_backward(zn_ctx *ctx, zn_loss loss, const float *output
 ZN_API zn_status zn_evaluate_classification(zn_ctx *ctx, const float *outputs, const float *targets, size_t rows,
                                             size_t cols, size_t num_classes, uint64_t *confusion, float *metrics4);
 
+/* ---- token models ------------------------------------------------------------------------ */
+/* The two ends of a network over tokens, beside the Dense path in between.  The reference has no such operators; what
+ * its conventions fix is kept: f32 at the boundary, row-major blocks, host or device pointers per operand, device
+ * operands only enqueue on the context's stream.  Device operands need not come from zn_tensor_alloc, but the call is
+ * ordered only behind earlier calls on this context: memory written on another stream has to be finished first.
+ *
+ * Token ids are int32.  A NEGATIVE id means "no token" (padding).  An id >= vocab is an error in the data: it reads
+ * and writes nothing out of range, its row gets what the entry point says below, and the next call that waits for the
+ * device (zn_end_command_batch, zn_tensor_download, any call with a host operand) returns ZN_ERR_INVALID_VALUE.
+ *
+ * Blocks of logits have a row pitch `ld` >= vocab in floats; columns from vocab to ld are neither read nor written.
+ * Outputs may not overlap inputs or each other unless an entry point says so (ZN_ERR_INVALID_VALUE).  rows == 0 does
+ * nothing, except that zn_embedding_backward still clears the table it was to write.  All sums, maxima and softmax statistics are formed in f32 whatever the context's precision mode, each in a
+ * fixed order: the same call gives the same bits. */
+
+/* Embedding lookup, a Dense layer on one-hot rows without the product: out[r][:] = scale * table[tokens[r]][:].
+ * table: vocab x dim, out: rows x dim, dense.  A row without a token, and one whose id is >= vocab, becomes zero. */
+ZN_API zn_status zn_embedding_forward(zn_ctx *ctx, const float *table, const int32_t *tokens, float *out, size_t rows,
+                                      size_t vocab, size_t dim, float scale);
+/* Its gradient: grad_table[t][:] (+)= scale * sum over the rows r with tokens[r] == t of grad_out[r][:], the rows of a
+ * token added in an order that depends on `tokens` and the sizes alone.  accumulate == 0 writes the whole table (zero
+ * where no row has the token); accumulate != 0 adds to it and leaves the rows of other tokens untouched.  Rows without
+ * a token, and ids >= vocab, add nothing. */
+ZN_API zn_status zn_embedding_backward(zn_ctx *ctx, const float *grad_out, const int32_t *tokens, float *grad_table,
+                                       size_t rows, size_t vocab, size_t dim, float scale, int32_t accumulate);
+
+/* Scores of every row of logits x at a temperature T > 0, with p = softmax(x / T):
+ *   logprob[r]      = log p[tokens[r]]; 0 without a token, NaN for an id >= vocab
+ *   entropy[r]      = -sum p log p (a column of probability 0 adds nothing)
+ *   row_stats[r]    = {max x, log sum exp((x - max x) / T)}: log p[c] = (x[c] - max x) / T - row_stats[r][1]
+ *   top_tokens[r][j], top_logprobs[r][j] = the j-th largest logit's column and log p, j < top_k <= 128; among equal
+ *                     logits the lowest column first.  A column at -inf is no alternative: such a place, and one past
+ *                     the vocabulary, holds -1 and -inf.
+ * A row whose logits are all -inf: logprob -inf (0 without a token), entropy 0, row_stats {-inf, -inf}, no
+ * alternatives.  A row with a NaN or +inf: NaN everywhere (also without a token), alternatives -1 and NaN.
+ * tokens and logprob go together, as do top_tokens, top_logprobs and top_k > 0; each of these pairs and each other
+ * output may be null, but not all of them. */
+ZN_API zn_status zn_token_logprobs(zn_ctx *ctx, const float *logits, size_t ld, const int32_t *tokens, size_t rows,
+                                   size_t vocab, float temperature, size_t top_k, float *logprob, float *entropy,
+                                   float *row_stats, int32_t *top_tokens, float *top_logprobs);
+/* Gradient of sum_r grad_logprob[r] logprob[r] + grad_entropy[r] entropy[r] with respect to the logits, from the
+ * row_stats and entropy of zn_token_logprobs at the same temperature:
+ *   grad[r][c] = ( grad_logprob[r] ([c == tokens[r]] - p[c]) - grad_entropy[r] p[c] (log p[c] + entropy[r]) ) / T
+ * grad_logprob (with tokens) or grad_entropy (with entropy) may be null.  A row without a token, or with an id >=
+ * vocab, has no logprob term.  A row whose factors are both zero gets zeros whatever it holds, a row whose logits are
+ * all -inf gets zeros, any other row with a NaN or +inf gets NaN.  grad_logits may be the logits themselves with
+ * ld_grad == ld. */
+ZN_API zn_status zn_token_logprobs_backward(zn_ctx *ctx, const float *logits, size_t ld, const int32_t *tokens,
+                                            const float *row_stats, const float *entropy, const float *grad_logprob,
+                                            const float *grad_entropy, float *grad_logits, size_t ld_grad, size_t rows,
+                                            size_t vocab, float temperature);
+
+/* Distillation from a teacher's top logits, loss and gradient in one call.  Row r of teacher_tokens / teacher_logits
+ * (rows x k, dense, k <= 512) lists tokens with their logits u (log-probabilities will do: a constant of the row does
+ * not matter); a negative token or a logit of -inf is no entry.  With q = softmax(u / T) over the entries, p =
+ * softmax(x / T) over the vocabulary and w = row_weights[r] (1 where row_weights is null):
+ *   row_loss[r] = w T^2 sum_j q_j (log q_j - log p[id_j])
+ *   grad[r][c]  = w T (p[c] - sum of q_j over the entries with id_j == c), the gradient of sum_r row_loss[r]
+ * An id listed twice counts twice.  A row of weight 0, and one without entries, has loss 0 and gradient 0 whatever its
+ * logits hold.  An entry whose logit x is -inf makes the loss +inf (where all of a row's are, its p counts as 0); a
+ * NaN or +inf in a row's logits or entries makes its loss and gradient NaN; an id >= vocab makes its loss NaN and its
+ * gradient zero.  row_loss or grad_logits may be null, not both; grad_logits may be the logits themselves with
+ * ld_grad == ld. */
+ZN_API zn_status zn_distill_loss(zn_ctx *ctx, const float *logits, size_t ld, const int32_t *teacher_tokens,
+                                 const float *teacher_logits, size_t rows, size_t vocab, size_t k, float temperature,
+                                 const float *row_weights, float *row_loss, float *grad_logits, size_t ld_grad);
+
+/* 4-bit weights.  Column j of a weight matrix w[k x n] is cut into groups of `group` (32, 64 or 128) rows, the last one
+ * shorter where k is not a multiple; w[i][j] ~ scales[j][i / group] * (code - 8), code in 0..15.
+ *   scales: n x ceil(k / group) floats
+ *   packed: n x 16 ceil(k / 128) 32-bit words, 16-byte aligned on the device.  A word holds eight codes, the lowest bits
+ *           first; in each run of 16 words (128 codes) the word of codes 8 (4 i + t) .. 8 (4 i + t) + 7 stands at place
+ *           4 t + i (i, t = 0..3).  Codes past k are ignored.
+ * zn_quantize4 takes the scale max |w| / 7 of each group and the nearest code, 1..15 (halves to even); codes past k are
+ * 8.  A group with a NaN or infinity gets a NaN scale and codes of 8. */
+ZN_API zn_status zn_quantize4(zn_ctx *ctx, const float *w, uint32_t *packed, float *scales, size_t n, size_t k,
+                              size_t group);
+/* The form of zn_matmul_bias_act for few rows: y[rows x n] = act(x[rows x k] . w + bias) on 4-bit weights.  bias may be
+ * null.  x enters with all its 24 significant bits, sums are f32.  Any number of rows is taken, sixteen at a time (each
+ * sixteen read the weights once). */
+ZN_API zn_status zn_matmul4_bias_act(zn_ctx *ctx, const float *x, const uint32_t *packed, const float *scales,
+                                     const float *bias, float *y, size_t rows, size_t n, size_t k, size_t group,
+                                     zn_activation act);
+/* The launch that a token-model operator would get, or the status with which its sizes are refused.  Host arithmetic
+ * only, no device needed.  op: 0 embedding_forward (rows, vocab, dim), 1 embedding_backward (rows, vocab, dim),
+ * 2 token_logprobs (rows, vocab, top_k), 3 token_logprobs_backward (rows, vocab, -), 4 distill_loss (rows, vocab, k),
+ * 5 quantize4 (n, k, group), 6 matmul4 (rows, n, k; group taken as valid).  out[0] = blocks, out[1] = threads per
+ * block, out[2] = blocks that share one row (or one table piece, or one column tile), out[3] = dynamic shared memory
+ * in bytes, out[4] = floats of scratch. */
+ZN_API zn_status zn_debug_token_plan(int32_t op, size_t a, size_t b, size_t c, int32_t sm_count, int64_t out[5]);
+
 /* ---- optimizers ------------------------------------------------------------------ */
 /* Backend.sgdUpdate, src/backend.zig:420-430 -> cpuSgdUpdate :2722-2739 (clamps included). */
 ZN_API zn_status zn_sgd_update(zn_ctx *ctx, float *weights, const float *grads, size_t count,

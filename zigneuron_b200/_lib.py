@@ -67,6 +67,14 @@ SIGNATURES = {
     "zn_adam_update": (i32, [vp, vp, vp, vp, vp, sz, f32, f32, f32, f32, f32, f32]),
     "zn_evaluate_classification": (i32, [vp, vp, vp, sz, sz, sz, vp, vp]),
     "zn_rmsprop_update": (i32, [vp, vp, vp, vp, sz, f32, f32, f32]),
+    "zn_embedding_forward": (i32, [vp, vp, vp, vp, sz, sz, sz, f32]),
+    "zn_embedding_backward": (i32, [vp, vp, vp, vp, sz, sz, sz, f32, i32]),
+    "zn_token_logprobs": (i32, [vp, vp, sz, vp, sz, sz, f32, sz, vp, vp, vp, vp, vp]),
+    "zn_token_logprobs_backward": (i32, [vp, vp, sz, vp, vp, vp, vp, vp, vp, sz, sz, sz, f32]),
+    "zn_distill_loss": (i32, [vp, vp, sz, vp, vp, sz, sz, sz, f32, vp, vp, vp, sz]),
+    "zn_quantize4": (i32, [vp, vp, vp, vp, sz, sz, sz]),
+    "zn_matmul4_bias_act": (i32, [vp, vp, vp, vp, vp, vp, sz, sz, sz, sz, i32]),
+    "zn_debug_token_plan": (i32, [i32, sz, sz, sz, i32, C.POINTER(C.c_int64)]),
     "zn_clip_grad_norm": (i32, [vp, pvp, psz, sz, pf, pf]),
     "zn_net_create": (i32, [vp, i32, pvp]),
     "zn_net_destroy": (None, [vp]),
@@ -118,13 +126,13 @@ for _name, (_res, _args) in SIGNATURES.items():
     _fn.restype, _fn.argtypes = _res, _args
 
 
-def ptr(x):
+def ptr(x, dtype=np.float32):
     """void* for a numpy array (host), a DeviceTensor, an int device address, or None."""
     if x is None:
         return None
     if isinstance(x, np.ndarray):
-        if x.dtype != np.float32 or not x.flags["C_CONTIGUOUS"]:
-            raise TypeError("operands must be C-contiguous float32 arrays")
+        if x.dtype != dtype or not x.flags["C_CONTIGUOUS"]:
+            raise TypeError(f"operands must be C-contiguous {np.dtype(dtype).name} arrays")
         return x.ctypes.data
     if hasattr(x, "address"):
         return x.address

@@ -39,23 +39,26 @@ class Loss(enum.IntEnum):            # order of src/loss.zig:12-22
 
 
 class DeviceTensor:
-    """A float32 block resident on the GPU (Tensor.init + its device handle, src/tensor.zig:17-118)."""
+    """A float32 block resident on the GPU (Tensor.init + its device handle, src/tensor.zig:17-118).  `dtype` may be
+    another four-byte type (int32 token ids, uint32 packed weights): the block's bytes are the same."""
 
-    def __init__(self, backend, count):
-        self.backend, self.count = backend, int(count)
+    def __init__(self, backend, count, dtype=np.float32):
+        self.backend, self.count, self.dtype = backend, int(count), np.dtype(dtype)
+        if self.dtype.itemsize != 4:
+            raise TypeError("device tensors hold four-byte values")
         out = C.c_void_p()
         check(lib.zn_tensor_alloc(backend.handle, self.count, C.byref(out)), backend.handle)
         self.address = out.value
 
     @classmethod
-    def from_numpy(cls, backend, array):
-        a = np.ascontiguousarray(array, dtype=np.float32)
-        t = cls(backend, a.size)
+    def from_numpy(cls, backend, array, dtype=np.float32):
+        a = np.ascontiguousarray(array, dtype=dtype)
+        t = cls(backend, a.size, dtype)
         check(lib.zn_tensor_upload(backend.handle, t.address, a.ctypes.data, a.size), backend.handle)
         return t
 
     def numpy(self, shape=None):
-        out = np.empty(self.count, np.float32)
+        out = np.empty(self.count, self.dtype)
         check(lib.zn_tensor_download(self.backend.handle, out.ctypes.data, self.address, self.count), self.backend.handle)
         return out.reshape(shape) if shape is not None else out
 
@@ -99,10 +102,10 @@ class Backend:
         self.precision = Precision(precision)
         self._ck(lib.zn_ctx_set_precision(self.handle, int(precision)))
 
-    def tensor(self, array_or_count):
+    def tensor(self, array_or_count, dtype=np.float32):
         if isinstance(array_or_count, (int, np.integer)):
-            return DeviceTensor(self, array_or_count)
-        return DeviceTensor.from_numpy(self, array_or_count)
+            return DeviceTensor(self, array_or_count, dtype)
+        return DeviceTensor.from_numpy(self, array_or_count, dtype)
 
     # ---- src/backend.zig:105-136
     def beginCommandBatch(self):
@@ -195,6 +198,52 @@ class Backend:
         self._ck(lib.zn_evaluate_classification(self.handle, ptr(outputs), ptr(targets), rows, cols, num_classes,
                                                 cm.ctypes.data, m.ctypes.data))
         return cm, dict(zip(("accuracy", "precision", "recall", "f1_score"), (float(v) for v in m)))
+
+    # ---- token models.  Token ids are int32, negative for "no token"; see include/zn_b200.h for every definition.
+    def embeddingForward(self, table, tokens, out, rows, vocab, dim, scale=1.0):
+        """out[r] = scale * table[tokens[r]]"""
+        self._ck(lib.zn_embedding_forward(self.handle, ptr(table), ptr(tokens, np.int32), ptr(out), rows, vocab, dim, scale))
+
+    def embeddingBackward(self, grad_out, tokens, grad_table, rows, vocab, dim, scale=1.0, accumulate=False):
+        """grad_table[t] (+)= scale * sum of grad_out[r] over the rows r of token t"""
+        self._ck(lib.zn_embedding_backward(self.handle, ptr(grad_out), ptr(tokens, np.int32), ptr(grad_table), rows, vocab, dim,
+                                           scale, int(accumulate)))
+
+    def tokenLogProbs(self, logits, tokens, rows, vocab, logprob=None, entropy=None, row_stats=None, top_k=0, top_tokens=None,
+                      top_logprobs=None, temperature=1.0, ld=None):
+        """Per row of logits / temperature: log-probability of tokens[r], entropy, {max, log-sum-exp less the max}, and the
+        top_k largest with their log-probabilities (-1 and -inf where there are fewer).  Outputs left out are not formed."""
+        self._ck(lib.zn_token_logprobs(self.handle, ptr(logits), vocab if ld is None else ld, ptr(tokens, np.int32), rows, vocab,
+                                       temperature, top_k, ptr(logprob), ptr(entropy), ptr(row_stats), ptr(top_tokens, np.int32),
+                                       ptr(top_logprobs)))
+
+    def tokenLogProbsBackward(self, logits, tokens, row_stats, entropy, grad_logprob, grad_entropy, grad_logits, rows, vocab,
+                              temperature=1.0, ld=None, ld_grad=None):
+        """Gradient of sum grad_logprob * logprob + grad_entropy * entropy with respect to the logits (in place allowed)."""
+        self._ck(lib.zn_token_logprobs_backward(self.handle, ptr(logits), vocab if ld is None else ld, ptr(tokens, np.int32),
+                                                ptr(row_stats), ptr(entropy), ptr(grad_logprob), ptr(grad_entropy), ptr(grad_logits),
+                                                vocab if ld_grad is None else ld_grad, rows, vocab, temperature))
+
+    def distillLoss(self, logits, teacher_tokens, teacher_logits, rows, vocab, k, temperature=1.0, row_weights=None, row_loss=None,
+                    grad_logits=None, ld=None, ld_grad=None):
+        """row_loss[r] = w T^2 KL(softmax of the teacher's k logits || softmax of the row), and its gradient (in place allowed)."""
+        self._ck(lib.zn_distill_loss(self.handle, ptr(logits), vocab if ld is None else ld, ptr(teacher_tokens, np.int32),
+                                     ptr(teacher_logits), rows, vocab, k, temperature, ptr(row_weights), ptr(row_loss),
+                                     ptr(grad_logits), vocab if ld_grad is None else ld_grad))
+
+    @staticmethod
+    def packed4_shape(n, k, group):
+        """Shapes of the packed words (uint32) and the scales (float32) of a k x n weight matrix."""
+        return (n, -(-k // 128) * 16), (n, -(-k // group))
+
+    def quantize4(self, w, packed, scales, n, k, group):
+        """Weights w[k x n] as 4-bit codes with one scale per `group` rows of a column."""
+        self._ck(lib.zn_quantize4(self.handle, ptr(w), ptr(packed, np.uint32), ptr(scales), n, k, group))
+
+    def matMul4BiasAct(self, x, packed, scales, bias, y, rows, n, k, group, act):
+        """y = act(x . w + bias) on the 4-bit weights; bias may be None.  Meant for few rows (16 share one read of w)."""
+        self._ck(lib.zn_matmul4_bias_act(self.handle, ptr(x), ptr(packed, np.uint32), ptr(scales), ptr(bias), ptr(y), rows, n, k,
+                                         group, int(Activation(act))))
 
     # ---- optimizers, src/backend.zig:420-443, :640-646
     def sgdUpdate(self, weights, gradients, learning_rate, weight_decay):

@@ -7,9 +7,7 @@
 
 #include "zn_internal.h"
 
-namespace {
-
-zn_status stage_reserve(zn_ctx *ctx, int slot, size_t floats) {
+zn_status zn_stage_reserve(zn_ctx *ctx, int slot, size_t floats) {
     if (ctx->stage_floats[slot] >= floats) return ZN_OK;
     ZN_CUDA(ctx, cudaStreamSynchronize(ctx->stream));
     cudaFree(ctx->stage[slot]);
@@ -19,6 +17,10 @@ zn_status stage_reserve(zn_ctx *ctx, int slot, size_t floats) {
     ctx->stage_floats[slot] = floats;
     return ZN_OK;
 }
+
+namespace {
+
+zn_status stage_reserve(zn_ctx *ctx, int slot, size_t floats) { return zn_stage_reserve(ctx, slot, floats); }
 
 // Resolves one operand: device pointers pass through, host pointers are staged in `slot`.
 struct Operand {

@@ -115,7 +115,7 @@ extern "C" void zn_ctx_destroy(zn_ctx *ctx) {
         if (ctx->lanes[i].stream) cudaStreamSynchronize(ctx->lanes[i].stream);
     if (ctx->dp) zn_dp_destroy(ctx);
     for (auto &kv : ctx->tensors) cudaFree(kv.first);
-    for (int i = 0; i < 6; ++i) cudaFree(ctx->stage[i]);
+    for (float *block : ctx->stage) cudaFree(block);
     cudaFree(ctx->scratch);
     cudaFree(ctx->tile_counters);
     cudaFree(ctx->block_counters);
@@ -149,6 +149,8 @@ zn_status zn_check_device_status(zn_ctx *ctx) {
     if (ctx->status_host && *ctx->status_host != 0) {
         int code = *ctx->status_host;
         *ctx->status_host = 0;
+        if (code == ZN_DEVICE_BAD_TOKEN)
+            return zn_fail(ctx, ZN_ERR_INVALID_VALUE, "an earlier call met a token id outside the vocabulary");
         return zn_fail(ctx, ZN_ERR_TIMEOUT, "a bounded device-side wait gave up (code %d)", code);
     }
     return ZN_OK;

@@ -26,6 +26,8 @@ struct zn_trace_rec { int family, lane; cudaEvent_t e0, e1; };   // one launch o
 
 struct zn_dp_state;   // dp.cu
 
+enum { ZN_STAGE_SLOTS = 10 };
+
 struct zn_ctx {
     int device = 0;
     int sm_count = 148;
@@ -53,8 +55,8 @@ struct zn_ctx {
     cudaStream_t opt_stream = nullptr, aux_stream = nullptr;
     cudaEvent_t lane_join[4] = {nullptr, nullptr, nullptr, nullptr};
     // Staging for ops called with host pointers; grown on demand.
-    float *stage[6] = {nullptr, nullptr, nullptr, nullptr, nullptr, nullptr};
-    size_t stage_floats[6] = {0, 0, 0, 0, 0, 0};
+    float *stage[ZN_STAGE_SLOTS] = {};
+    size_t stage_floats[ZN_STAGE_SLOTS] = {};
     float *pinned_scalar = nullptr;       // 16 floats of pinned host memory for scalar read-backs
 
     std::unordered_map<float *, size_t> tensors;   // zn_tensor_alloc registry (ptr -> count)
@@ -143,6 +145,9 @@ zn_status zn_sync_all_lanes(zn_ctx *ctx);         // host waits for every lane
 zn_status zn_join_lanes_into_main(zn_ctx *ctx);   // the main stream waits (on the device) for the other lanes
 
 zn_status zn_scratch_reserve(zn_ctx *ctx, size_t floats);
+zn_status zn_stage_reserve(zn_ctx *ctx, int slot, size_t floats);
+// What a kernel writes into the context's status word when a token id lies outside the vocabulary.
+enum { ZN_DEVICE_BAD_TOKEN = -1001 };
 // The active lane's 1024 arrival counters (allocated and cleared on first use); see zn_ctx::block_counters.
 enum { ZN_COUNTERS_PER_LANE = 1024, ZN_COUNTER_SUMSQ = 1000, ZN_COUNTER_LOSS = 1001 };   // [0, 1000): column strips
 zn_status zn_lane_counters(zn_ctx *ctx, unsigned int **out);
@@ -240,3 +245,42 @@ zn_status zn_k_sgd(zn_ctx *ctx, const zn_opt_args &a, bool is_bias);
 zn_status zn_k_adam(zn_ctx *ctx, const zn_opt_args &a);
 zn_status zn_k_sgd_momentum(zn_ctx *ctx, const zn_opt_args &a);
 zn_status zn_k_rmsprop(zn_ctx *ctx, const zn_opt_args &a);
+
+// ---- token models (each launcher enqueues on ctx->stream; sizes and pointers have been checked) ----------------
+
+struct zn_token_plan { int64_t blocks = 0; int threads = 0; int share = 1; size_t smem = 0; size_t scratch_floats = 0; };
+enum { ZN_TOP_MAX = 128, ZN_TEACHER_MAX = 512 };
+
+zn_token_plan zn_plan_embedding_forward(size_t rows, size_t dim, int sms);
+zn_status zn_k_embedding_forward(zn_ctx *ctx, const float *table, const int32_t *tokens, float *out, size_t rows, size_t vocab,
+                                 size_t dim, float scale);
+zn_token_plan zn_plan_embedding_backward(size_t rows, size_t vocab, size_t dim, int sms);
+zn_status zn_k_embedding_backward(zn_ctx *ctx, const float *grad_out, const int32_t *tokens, float *grad_table, size_t rows,
+                                  size_t vocab, size_t dim, float scale, bool accumulate);
+
+struct zn_scores_args {
+    const float *logits; int64_t ld; const int32_t *tokens; int64_t rows, vocab; float temperature; int top_k;
+    float *logprob, *entropy, *stats; int32_t *top_tokens; float *top_logprobs;
+};
+zn_token_plan zn_plan_token_logprobs(size_t rows, size_t vocab, size_t top_k, int sms);
+zn_status zn_k_token_logprobs(zn_ctx *ctx, const zn_scores_args &a);
+
+struct zn_scores_grad_args {
+    const float *logits; int64_t ld; const int32_t *tokens; const float *stats, *entropy, *grad_logprob, *grad_entropy;
+    float *grad; int64_t ld_grad; int64_t rows, vocab; float temperature;
+};
+zn_token_plan zn_plan_token_logprobs_backward(size_t rows, size_t vocab, int sms);
+zn_status zn_k_token_logprobs_backward(zn_ctx *ctx, const zn_scores_grad_args &a);
+
+struct zn_distill_args {
+    const float *logits; int64_t ld; const int32_t *ids; const float *teacher; int64_t rows, vocab; int k; float temperature;
+    const float *weights; float *loss; float *grad; int64_t ld_grad;
+};
+zn_token_plan zn_plan_distill(size_t rows, size_t vocab, size_t k, int sms);
+zn_status zn_k_distill(zn_ctx *ctx, const zn_distill_args &a);
+
+zn_token_plan zn_plan_quantize4(size_t n, size_t k, int sms);
+zn_status zn_k_quantize4(zn_ctx *ctx, const float *w, uint32_t *packed, float *scales, size_t n, size_t k, size_t group);
+zn_token_plan zn_plan_matmul4(size_t rows, size_t n, size_t k, int sms);
+zn_status zn_k_matmul4(zn_ctx *ctx, const float *x, const uint32_t *packed, const float *scales, const float *bias, float *y,
+                       size_t rows, size_t n, size_t k, size_t group, int act);
