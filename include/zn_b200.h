@@ -194,7 +194,7 @@ ZN_API zn_status zn_embedding_forward(zn_ctx *ctx, const float *table, const int
 ZN_API zn_status zn_embedding_backward(zn_ctx *ctx, const float *grad_out, const int32_t *tokens, float *grad_table,
                                        size_t rows, size_t vocab, size_t dim, float scale, int32_t accumulate);
 
-/* Scores of every row of logits x at a temperature T > 0, with p = softmax(x / T):
+/* Scores of every row of logits x at a temperature T (1e-4 to 1e4), with p = softmax(x / T):
  *   logprob[r]      = log p[tokens[r]]; 0 without a token, NaN for an id >= vocab
  *   entropy[r]      = -sum p log p (a column of probability 0 adds nothing)
  *   row_stats[r]    = {max x, log sum exp((x - max x) / T)}: log p[c] = (x[c] - max x) / T - row_stats[r][1]

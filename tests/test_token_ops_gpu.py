@@ -663,7 +663,7 @@ def test_refusals(be):
     refused(INVALID, be.tokenLogProbs, f, None, 2, 8, entropy=o, row_stats=o)        # two outputs on one another
     refused(SHAPE, be.tokenLogProbs, f, None, 2, 8, entropy=o, ld=7)
     refused(SHAPE, be.tokenLogProbs, f, None, 2, 0, entropy=o)
-    for t in (0.0, -1.0, np.inf, np.nan):
+    for t in (0.0, -1.0, np.inf, np.nan, 9e-5, 1.1e4):
         refused(INVALID, be.tokenLogProbs, f, None, 2, 8, entropy=o, temperature=t)
         refused(INVALID, be.tokenLogProbsBackward, f, i, f, None, f, None, o, 2, 8, t)
         refused(INVALID, be.distillLoss, f, i, f, 2, 8, 2, t, grad_logits=o)
