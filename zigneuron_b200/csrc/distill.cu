@@ -1,234 +1,431 @@
 // Distillation from a teacher's top logits: loss and gradient of a row in one pass over it.
 //
-// The row is read from HBM once and the gradient written once: a cluster of blocks holds the row in shared memory, each
-// block a slice of it.  While a slice comes in, each thread keeps the softmax statistics of what it loads; the slices'
-// statistics are exchanged through distributed shared memory, and the gradient is formed from the copy on chip.
-#include <cooperative_groups.h>
-
-#include <utility>
-
+// The row is read from HBM once and the gradient written once.  A cluster of blocks holds a row, each block a slice of it,
+// and goes from row to row.  In a block a ring of buffers keeps the next rows on their way (bulk copies) while one is
+// worked on.  Each thread takes its values of the slice to registers and turns them into exponentials against its own
+// maximum, so that one exponential per value does for the sums and the gradient both; every warp sends its maximum and
+// sum to all blocks of the row through distributed shared memory; the gradient, a product per value, goes back to the
+// buffer, and from there out by a bulk copy.  What is slow and small -- the teacher's entries, the listed tokens, the
+// loss -- is left to helper warps.
 #include "zn_token.cuh"
 
 namespace {
 
-namespace cg = cooperative_groups;
-constexpr int TPB = 256;
-constexpr int MAX_SHARE = 8;
+constexpr int MAX_SHARE = 8, MAX_RING = 3, MAX_WARPS = 16;
+constexpr int HELD = 36;                         // values of a slice that a thread holds in registers
 
 struct Shared {
-    zn_softmax part[TPB / 32];
-    zn_softmax slice[MAX_SHARE];                 // statistics of every slice of the row, in their order
-    float q[ZN_TEACHER_MAX], x[ZN_TEACHER_MAX];  // the teacher's probability and the student's logit of an entry
-    int32_t id[ZN_TEACHER_MAX];                  // its token, -1 for no entry
-    float loss_q, ubad;
-    int wrong, some;
+    float warp[2][MAX_SHARE * MAX_WARPS][2];     // maximum and sum of every warp of the row's blocks; rows take turns
+    float ends[MAX_RING][8];                     // the values before and behind the aligned part of the slice
+    float weight[MAX_RING], loss_q[MAX_RING];    // sum q log q of the row in this place of the ring
+    int state[MAX_RING];                         // what the teacher's entries leave of it
+    float m[MAX_RING], s[MAX_RING];              // what the row comes to
+    int verdict[MAX_RING], copy_out[MAX_RING];   // the gradient stands in the ring and goes out by a copy
+    uint64_t full[MAX_RING], done[MAX_RING], free_[MAX_RING], met[2];
 };
+enum { FILL_GRADIENT = 0, FILL_ZERO = 1, FILL_NAN = 2, FILL_EMPTY = 3 };
+enum { ROW_FINE = 0, ROW_NONE = 1, ROW_WRONG = 2, ROW_NAN = 3 };     // nothing to learn; id past the vocabulary; NaN among the logits
 
-// The teacher's entries of a row, by one warp: q = softmax(u / T) over them.
-__device__ void read_teacher(Shared &s, const zn_distill_args &a, int64_t r, const float *x, int lane, bool report, int *status) {
+// The teacher's entries of a row, by one warp: q = softmax(u / T) over them, the student's logits at their tokens.
+__device__ void read_teacher(const zn_distill_args &a, int64_t r, int lane, float *q, float *xt, int32_t *id, float *together, float *loss_q,
+                             int *state, bool report, int *status) {
+    const float *x = a.logits + r * a.ld;
     const float inv_t = 1.f / a.temperature;
     float um = -INFINITY;
-    bool wrong = false, ubad = false;
+    bool wrong = false, nan = false;
     for (int j = lane; j < a.k; j += 32) {
         const int32_t t = a.ids[r * a.k + j];
         const float u = a.teacher[r * a.k + j];
         const bool entry = t >= 0 && u != -INFINITY;
         wrong = wrong || (entry && t >= a.vocab);
-        ubad = ubad || (entry && !(u < INFINITY));
+        nan = nan || (entry && !(u < INFINITY));
         const bool fine = entry && t < a.vocab;
-        s.id[j] = fine ? t : -1;
-        s.x[j] = fine ? x[t] : 0.f;
-        s.q[j] = u;
+        id[j] = fine ? t : -1;
+        xt[j] = fine ? x[t] : 0.f;
+        q[j] = u;
         if (entry) um = fmaxf(um, u);
     }
     um = zn_warp_max(um);
     wrong = __any_sync(0xffffffffu, wrong);
-    ubad = __any_sync(0xffffffffu, ubad);
+    nan = __any_sync(0xffffffffu, nan);
     if (wrong && report && lane == 0) zn_bad_token(status);
     const float c = 1.4426950408889634f * inv_t;
     float mass = 0.f;
     for (int j = lane; j < a.k; j += 32)
-        if (s.id[j] >= 0) mass += zn_exp2((s.q[j] - um) * c);
+        if (id[j] >= 0) mass += zn_exp2((q[j] - um) * c);
     mass = zn_warp_sum(mass);
     const float inv_mass = 1.f / mass, log_mass = logf(mass);
-    float lq = 0.f;                              // sum q log q
+    float lq = 0.f;
     for (int j = lane; j < a.k; j += 32) {
-        const float d = s.q[j] - um, q = s.id[j] >= 0 ? zn_exp2(d * c) * inv_mass : 0.f;
-        if (q > 0.f) lq += q * (d * inv_t - log_mass);
-        s.q[j] = q;
+        const float d = q[j] - um, p = id[j] >= 0 ? zn_exp2(d * c) * inv_mass : 0.f;
+        if (p > 0.f) lq += p * (d * inv_t - log_mass);
+        q[j] = p;
     }
     lq = zn_warp_sum(lq);
+    __syncwarp();
+    // The first place of an id takes the q of all its places, in their order; the others are taken out.  Few rows list an
+    // id twice, so the sums are formed where one is found only.
+    for (int j0 = 0; j0 < a.k; j0 += 32) {
+        const int j = j0 + lane;
+        const int32_t mine = j < a.k ? id[j] : -1;
+        int same = 0;
+#pragma unroll 8
+        for (int i = 0; i < a.k; ++i) same += id[i] == mine;
+        float sum = mine >= 0 ? q[j] : -1.f;
+        if (mine >= 0 && same > 1) {
+            int before = 0;
+            sum = 0.f;
+            for (int i = 0; i < a.k; ++i)
+                if (id[i] == mine) {
+                    before += i < j;
+                    sum += q[i];
+                }
+            if (before > 0) sum = -1.f;
+        }
+        if (j < a.k) together[j] = sum;
+    }
     if (lane == 0) {
-        s.loss_q = lq;
-        s.ubad = ubad ? 1.f : 0.f;
-        s.wrong = wrong;
-        s.some = um > -INFINITY || ubad;
+        *loss_q = lq;
+        *state = wrong ? ROW_WRONG : nan ? ROW_NAN : um == -INFINITY ? ROW_NONE : ROW_FINE;
     }
 }
 
-// Stores n values from i = 0 on: four at a time by vec(i) from `from` on where g and the copy on chip stand alike on 16
-// bytes, one at a time by one(i) elsewhere (neighbouring lanes take neighbouring values: whole lines, no bank conflicts).
-template <typename V, typename F>
-__device__ __forceinline__ void store_slice(float *g, int64_t n, int64_t from, V vec, F one) {
-    int64_t lo = 0;
-    if (((reinterpret_cast<uintptr_t>(g + from)) & 15) == 0) {
-        const int64_t vecs = (n - from) / 4;
-#pragma unroll 4
-        for (int64_t i = threadIdx.x; i < vecs; i += TPB) __stcs(reinterpret_cast<float4 *>(g + from + 4 * i), vec(from + 4 * i));
-        if (threadIdx.x < from) g[threadIdx.x] = one(threadIdx.x);
-        lo = from + 4 * vecs;
-    }
-#pragma unroll 4
-    for (int64_t i = lo + threadIdx.x; i < n; i += TPB) __stcs(g + i, one(i));
+// n values of one kind.
+template <int THREADS>
+__device__ __forceinline__ void fill_slice(float *g, int n, float v) {
+    const int from = (int)zn_aligned_from(g, n), vecs = (n - from) / 4, to = from + 4 * vecs;
+    for (int i = threadIdx.x; i < vecs; i += THREADS) __stcs(reinterpret_cast<float4 *>(g + from + 4 * i), make_float4(v, v, v, v));
+    if (threadIdx.x < from) g[threadIdx.x] = v;
+    if (threadIdx.x < n - to) g[to + threadIdx.x] = v;
 }
 
-__global__ void __launch_bounds__(TPB) distill_kernel(zn_distill_args a, int share, int64_t slice, int64_t keep, int *status) {
-    extern __shared__ __align__(16) float kept[];          // the first `keep` values of the slice, shifted to the row's alignment
+// THREADS of arithmetic and five warps around them: one starts the copies in, one finishes rows and sends them out, and one
+// per place of the ring reads the teacher's entries (a chain of dependent reads and small sums, some microseconds long).
+// REGS: a slice fits in the threads' registers; else each value's exponential is formed twice.  WHOLE: it fits on chip;
+// else what does not is read twice.
+template <int THREADS, bool REGS, bool WHOLE>
+__global__ void __launch_bounds__(THREADS + 64 + 32 * MAX_RING) distill_kernel(zn_distill_args a, int share, int slice, int keep, int ring, int *status) {
+    extern __shared__ __align__(16) float dynamic[];       // ring x (keep + 4) logits, then ring x k of q, x, id, together
     __shared__ Shared s;
-    cg::cluster_group cluster = cg::this_cluster();
-    // before another block's shared memory is written it has to have started: the wait is far below
-    auto started = cluster.barrier_arrive();
-    const int64_t r = blockIdx.x / share;
-    const int rank = (int)(blockIdx.x % share);
-    const int64_t lo = min((int64_t)rank * slice, a.vocab), n = min(a.vocab, lo + slice) - lo;
-    const float *row = a.logits + r * a.ld, *x = row + lo;
-    const float w = a.weights ? a.weights[r] : 1.f, inv_t = 1.f / a.temperature, c = 1.4426950408889634f * inv_t, nan = zn_nan();
-    if (threadIdx.x < 32) read_teacher(s, a, r, row, threadIdx.x, rank == 0, status);
-    // the slice, and its statistics on the way
-    const int64_t from = zn_aligned_from(x, n), vecs = (n - from) / 4, to = from + 4 * vecs;
-    const int64_t shift = (4 - from) & 3;
-    zn_softmax st{-INFINITY, 0.f, 0.f};
-    if (w != 0.f) {
-        for (int64_t i0 = 0; i0 < vecs; i0 += 4 * TPB) {
-            float v[16];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int64_t i = i0 + j * TPB + threadIdx.x;
-                float4 f = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
-                if (i < vecs) f = *reinterpret_cast<const float4 *>(x + from + 4 * i);
-                v[4 * j] = f.x; v[4 * j + 1] = f.y; v[4 * j + 2] = f.z; v[4 * j + 3] = f.w;
-            }
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int64_t at = from + 4 * (i0 + j * TPB + threadIdx.x);
-                if (at + 4 <= keep && at < to)
-                    *reinterpret_cast<float4 *>(kept + shift + at) = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
-            }
-            zn_softmax_add<16, false>(st, v, c);
+    constexpr int WARPS = THREADS / 32;
+    const int rank = (int)(blockIdx.x % share), lane = threadIdx.x & 31;
+    const int64_t cluster = blockIdx.x / share, clusters = gridDim.x / share;
+    const int64_t lo = min((int64_t)rank * slice, a.vocab);
+    const int n = (int)(min(a.vocab, lo + slice) - lo);
+    const int pitch = keep + 4;
+    float *teacher = dynamic + ring * pitch;
+    const float inv_t = 1.f / a.temperature, c = 1.4426950408889634f * inv_t;
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < ring; ++i) {
+            zn_bar_init(&s.full[i], 3);
+            zn_bar_init(&s.done[i], WARPS);
+            zn_bar_init(&s.free_[i], 1);
         }
-        float v[1] = {-INFINITY};
-        int64_t end = -1;
-        if (threadIdx.x < from) end = threadIdx.x;
-        else if (threadIdx.x >= 32 && threadIdx.x - 32 < n - to) end = to + threadIdx.x - 32;
-        if (end >= 0) {
-            v[0] = x[end];
-            if (end < keep) kept[shift + end] = v[0];
-        }
-        zn_softmax_add<1, false>(st, v, c);
+        zn_bar_init(&s.met[0], 1);
+        zn_bar_init(&s.met[1], 1);
+        zn_bar_init_done();
     }
-    st = zn_softmax_block<TPB>(st, c, s.part);
-    cluster.barrier_wait(std::move(started));
-    if (share > 1) {
-        if (threadIdx.x < share) cluster.map_shared_rank(s.slice, threadIdx.x)[rank] = st;
-        cluster.sync();                          // also: nobody still reads logits that another block may now overwrite
-        st = s.slice[0];
-        for (int i = 1; i < share; ++i) zn_softmax_join(st, s.slice[i], c);
-    } else {
-        __syncthreads();
-    }
-    const bool bad = !(st.s >= 0.f) || s.ubad != 0.f, empty = st.m == -INFINITY;
-    const bool none = w == 0.f || s.wrong != 0 || !s.some;
-    const float ls = logf(st.s), inv_s = 1.f / st.s, wt = w * a.temperature;
-    if (a.loss && rank == 0 && threadIdx.x < 32) {
-        // sum q (log q - log p) = sum q log q - sum q log p
-        float lp = 0.f;
-        for (int j = threadIdx.x; j < a.k; j += 32)
-            if (s.q[j] > 0.f) lp += s.q[j] * (empty ? -INFINITY : (s.x[j] - st.m) * inv_t - ls);
-        lp = zn_warp_sum(lp);
-        if (threadIdx.x == 0) a.loss[r] = none ? (w != 0.f && s.wrong ? nan : 0.f) : bad ? nan : wt * a.temperature * (s.loss_q - lp);
-    }
-    if (!a.grad) return;
-    float *g = a.grad + r * a.ld_grad + lo;
-    if (none || bad || empty) {
-        const float fill = none ? 0.f : bad ? nan : 0.f;
-        store_slice(g, n, from, [&](int64_t) { return make_float4(fill, fill, fill, fill); }, [&](int64_t) { return fill; });
-    } else {
-        const float f = wt * inv_s;
-        const float *mine = kept + shift;
-        const auto p = [&](float v) { return f * zn_exp2((v - st.m) * c); };
-        const auto p4 = [&](const float *at) {
-            const float4 v = *reinterpret_cast<const float4 *>(at);
-            return make_float4(p(v.x), p(v.y), p(v.z), p(v.w));
-        };
-        const int64_t on_chip = n <= keep ? n : from + (keep - from) / 4 * 4;
-        if (n <= keep)
-            store_slice(g, n, from, [&](int64_t i) { return p4(mine + i); }, [&](int64_t i) { return p(mine[i]); });
-        else
-            store_slice(g, n, from, [&](int64_t i) { return p4(i < on_chip ? mine + i : x + i); },
-                        [&](int64_t i) { return p(i < on_chip ? mine[i] : x[i]); });
-    }
-    if (none || bad) return;
     __syncthreads();
-    // the listed tokens of this slice: the first place of an id takes the q of all its places
-    for (int j = threadIdx.x; j < a.k; j += TPB) {
-        const int32_t id = s.id[j];
-        if (id < lo || id >= lo + n) continue;
-        float sum = 0.f;
-        bool first = true;
-        for (int i = 0; i < a.k; ++i)
-            if (s.id[i] == id) {
-                if (i < j) first = false;
-                sum += s.q[i];
+    zn_cluster_arrive();         // every block has started before another one writes to its shared memory
+    zn_cluster_wait();
+    // The aligned part of the slice that fits on chip, from `from` on, `vecs` times four values; the ring holds it at the
+    // same place modulo 16 bytes.
+    const auto lay_out = [&](int64_t r, const float *&x, int &from, int &vecs, float *&mine, int place) {
+        x = a.logits + r * a.ld + lo;
+        from = (int)zn_aligned_from(x, n);
+        vecs = max(0, (min(n, keep) - from) / 4);
+        mine = dynamic + place * pitch + ((4 - from) & 3);
+    };
+    // the gradient at a listed token
+    const auto at_token = [&](float x, float m, float inv_s, float wt, float q) {
+        const float e = m == -INFINITY ? 0.f : zn_exp2(__fmul_rn(x - m, c));
+        return __fmul_rn(wt, __fmaf_rn(e, inv_s, -q));
+    };
+    const float *x;
+    float *mine;
+    int from, vecs;
+
+    if (threadIdx.x >= THREADS) {
+        const int helper = (threadIdx.x - THREADS) >> 5;
+        int place = 0, turn = 0;
+        for (int64_t r = cluster; r < a.rows; r += clusters) {
+            float *q = teacher + place * 4 * a.k, *xt = q + a.k, *together = q + 3 * a.k;
+            int32_t *id = reinterpret_cast<int32_t *>(q + 2 * a.k);
+            if (turn > 0 && (helper == place || helper == MAX_RING)) zn_bar_wait(&s.free_[place], (turn - 1) & 1, status, 21);
+            if (helper == place) {
+                read_teacher(a, r, lane, q, xt, id, together, &s.loss_q[place], &s.state[place], rank == 0, status);
+                __syncwarp();
+                if (lane == 0) zn_bar_arrive(&s.full[place]);
+            } else if (helper == MAX_RING) {
+                lay_out(r, x, from, vecs, mine, place);
+                const float w = a.weights ? a.weights[r] : 1.f;
+                if (lane == 0) {
+                    const uint32_t bytes = w == 0.f ? 0u : 16u * (uint32_t)vecs;
+                    zn_bar_expect(&s.full[place], bytes);
+                    // in four pieces, so that several copies are under way at once
+                    const uint32_t part = ((bytes + 63) / 64) * 16;
+                    for (uint32_t at = 0; at < bytes; at += part)
+                        zn_bulk_load(reinterpret_cast<char *>(mine + from) + at, reinterpret_cast<const char *>(x + from) + at, min(part, bytes - at),
+                                     &s.full[place]);
+                    s.weight[place] = w;
+                }
+                const int to = from + 4 * vecs, at = lane < 4 ? lane : to + lane - 4;
+                if (lane < 8) s.ends[place][lane] = w != 0.f && (lane < 4 ? at < from : at < n) ? x[at] : -INFINITY;
+                __syncwarp();
+                if (lane == 0) zn_bar_arrive(&s.full[place]);
+            } else if (helper == MAX_RING + 1) {
+                lay_out(r, x, from, vecs, mine, place);
+                zn_bar_wait(&s.done[place], turn & 1, status, 24);
+                const float m = s.m[place], sum = s.s[place], w = s.weight[place], wt = w * a.temperature;
+                const int verdict = s.verdict[place], to = from + 4 * vecs;
+                float *g = a.grad ? a.grad + r * a.ld_grad + lo : nullptr;
+                if (g && (verdict == FILL_GRADIENT || verdict == FILL_EMPTY)) {
+                    // the listed tokens of this slice; an id's first place has the q of all its places
+                    const float inv_s = verdict == FILL_EMPTY ? 0.f : 1.f / sum;
+                    for (int j = lane; j < a.k; j += 32) {
+                        const int64_t col = id[j] - lo;
+                        if (together[j] < 0.f || col < 0 || col >= n) continue;
+                        const float v = at_token(xt[j], m, inv_s, wt, together[j]);
+                        if (s.copy_out[place] && col >= from && col < to) mine[col] = v;
+                        else g[col] = v;
+                    }
+                }
+                // the values were written by ordinary stores, here and by the threads that arrived: the copy sees them after this
+                zn_async_fence();
+                __syncwarp();
+                if (lane == 0 && s.copy_out[place]) zn_bulk_store(g + from, mine + from, 16u * (uint32_t)vecs);
+                if (a.loss && rank == 0) {
+                    // sum q (log q - log p) = sum q log q - sum q log p
+                    const float ls = logf(sum);
+                    float lp = 0.f;
+                    for (int j = lane; j < a.k; j += 32)
+                        if (q[j] > 0.f) lp += q[j] * (m == -INFINITY ? -INFINITY : (xt[j] - m) * inv_t - ls);
+                    lp = zn_warp_sum(lp);
+                    if (lane == 0)
+                        a.loss[r] = verdict == FILL_ZERO ? (w != 0.f && s.state[place] == ROW_WRONG ? zn_nan() : 0.f)
+                                    : verdict == FILL_NAN ? zn_nan() : wt * a.temperature * (s.loss_q[place] - lp);
+                }
+                __syncwarp();
+                if (lane == 0) {
+                    zn_bulk_store_read();
+                    zn_bar_arrive(&s.free_[place]);
+                }
             }
-        if (first) g[id - lo] = wt * ((empty ? 0.f : zn_exp2((s.x[j] - st.m) * c) * inv_s) - sum);
+            if (++place == ring) {
+                place = 0;
+                ++turn;
+            }
+        }
+        __syncwarp();
+    } else {
+        int place = 0, phase = 0, side = 0, side_phase = 0;
+        for (int64_t r = cluster; r < a.rows; r += clusters) {
+            lay_out(r, x, from, vecs, mine, place);
+            const int on_chip = from + 4 * vecs;
+            zn_bar_wait(&s.full[place], phase, status, 22);
+            const int state = s.state[place];
+            const float w = s.weight[place];
+            // up to eight values outside the aligned part; -inf where there are fewer
+            const float end = threadIdx.x < 8 && w != 0.f ? s.ends[place][threadIdx.x] : -INFINITY;
+            float v[REGS ? HELD : 1];
+            zn_softmax st{-INFINITY, 0.f, 0.f};
+            if (REGS) {
+#pragma unroll
+                for (int j = 0; j < HELD / 4; ++j) {
+                    const int i = threadIdx.x + j * THREADS;
+                    float4 f = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+                    if (i < vecs && w != 0.f) f = *reinterpret_cast<const float4 *>(mine + from + 4 * i);
+                    v[4 * j] = f.x; v[4 * j + 1] = f.y; v[4 * j + 2] = f.z; v[4 * j + 3] = f.w;
+                    st.m = fmaxf(st.m, fmaxf(fmaxf(f.x, f.y), fmaxf(f.z, f.w)));
+                }
+                st.m = fmaxf(st.m, end);
+                const float base = st.m == -INFINITY ? 0.f : st.m;
+                float part[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int j = 0; j < HELD; ++j) {
+                    v[j] = zn_exp2(__fmul_rn(v[j] - base, c));
+                    part[j & 3] += v[j];
+                }
+                st.s = (part[0] + part[1]) + (part[2] + part[3]) + zn_exp2(__fmul_rn(end - base, c));
+            } else if (w != 0.f) {
+                int i = threadIdx.x;
+                for (; i + 3 * THREADS < vecs; i += 4 * THREADS) {
+                    float u[16];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const float4 f = *reinterpret_cast<const float4 *>(mine + from + 4 * (i + j * THREADS));
+                        u[4 * j] = f.x; u[4 * j + 1] = f.y; u[4 * j + 2] = f.z; u[4 * j + 3] = f.w;
+                    }
+                    zn_softmax_add<16, false>(st, u, c);
+                }
+                for (; i < vecs; i += THREADS) {
+                    const float4 f = *reinterpret_cast<const float4 *>(mine + from + 4 * i);
+                    const float u[4] = {f.x, f.y, f.z, f.w};
+                    zn_softmax_add<4, false>(st, u, c);
+                }
+                const float u[1] = {end};
+                zn_softmax_add<1, false>(st, u, c);
+                if (!WHOLE)         // up to four of them are in `ends` already
+                    for (int j = on_chip + 4 + threadIdx.x; j < n; j += THREADS) {
+                        const float o[1] = {x[j]};
+                        zn_softmax_add<1, false>(st, o, c);
+                    }
+            }
+            // over the warp, then over all warps of the row's blocks: each sends what it has to every block
+            const float own_m = st.m;
+            zn_softmax_raise<false>(st, zn_warp_max(st.m), c);
+            st.s = zn_warp_sum(st.s);
+            if (threadIdx.x == 0) zn_bar_expect(&s.met[side], 8u * WARPS * (uint32_t)share);
+            if (lane < share) zn_cluster_send(s.warp[side][rank * WARPS + (threadIdx.x >> 5)], st.m, st.s, &s.met[side], lane);
+            zn_bar_wait(&s.met[side], side_phase, status, 23);       // from here on nobody still needs the logits in global memory
+            const int all = share * WARPS;
+            float am[MAX_SHARE * WARPS / 32 + 1], m = -INFINITY, sum = 0.f;
+#pragma unroll
+            for (int j = 0; j < MAX_SHARE * WARPS / 32 + 1; ++j) {
+                const int i = lane + 32 * j;
+                am[j] = i < all ? s.warp[side][i][0] : -INFINITY;
+                m = fmaxf(m, am[j]);
+            }
+            m = zn_warp_max(m);
+#pragma unroll
+            for (int j = 0; j < MAX_SHARE * WARPS / 32 + 1; ++j) {
+                const int i = lane + 32 * j;
+                if (i < all) sum += s.warp[side][i][1] * zn_exp2(am[j] == m ? 0.f : __fmul_rn(am[j] - m, c));
+            }
+            sum = zn_warp_sum(sum);
+            side_phase ^= side;
+            side ^= 1;
+            const int verdict = w == 0.f || state == ROW_NONE || state == ROW_WRONG ? FILL_ZERO
+                                : !(sum >= 0.f) || state == ROW_NAN ? FILL_NAN : m == -INFINITY ? FILL_EMPTY : FILL_GRADIENT;
+            float *g = a.grad ? a.grad + r * a.ld_grad + lo : nullptr;
+            const bool copy_out = WHOLE && g && verdict == FILL_GRADIENT && ((reinterpret_cast<uintptr_t>(g + from)) & 15) == 0;
+            if (threadIdx.x == 0) {
+                s.m[place] = m;
+                s.s[place] = sum;
+                s.verdict[place] = verdict;
+                s.copy_out[place] = copy_out;
+            }
+            if (g && verdict == FILL_GRADIENT) {
+                const float f = __fmul_rn(w * a.temperature, 1.f / sum);
+                const auto p = [&](float u) { return __fmul_rn(f, zn_exp2(__fmul_rn(u - m, c))); };
+                if (REGS) {
+                    const float fe = __fmul_rn(f, zn_exp2(own_m == m ? 0.f : __fmul_rn(own_m - m, c)));
+#pragma unroll
+                    for (int j = 0; j < HELD / 4; ++j) {
+                        const int i = threadIdx.x + j * THREADS;
+                        if (i < vecs)
+                            *reinterpret_cast<float4 *>(mine + from + 4 * i) =
+                                make_float4(__fmul_rn(fe, v[4 * j]), __fmul_rn(fe, v[4 * j + 1]), __fmul_rn(fe, v[4 * j + 2]), __fmul_rn(fe, v[4 * j + 3]));
+                    }
+                } else {
+#pragma unroll 4
+                    for (int i = threadIdx.x; i < vecs; i += THREADS) {
+                        float4 *at = reinterpret_cast<float4 *>(mine + from + 4 * i);
+                        const float4 u = *at;
+                        *at = make_float4(p(u.x), p(u.y), p(u.z), p(u.w));
+                    }
+                    if (!WHOLE)
+                        for (int j = on_chip + 4 + threadIdx.x; j < n; j += THREADS) g[j] = p(x[j]);
+                }
+                if (threadIdx.x < 8) {
+                    const int at = threadIdx.x < 4 ? threadIdx.x : on_chip + threadIdx.x - 4;
+                    if (threadIdx.x < 4 ? at < from : at < n) g[at] = p(end);
+                }
+                if (!copy_out) {
+                    // the two blocks do not stand alike: neighbouring lanes take neighbouring values
+                    zn_part_sync(THREADS);
+#pragma unroll 4
+                    for (int i = from + threadIdx.x; i < on_chip; i += THREADS) __stcs(g + i, mine[i]);
+                }
+            } else if (g) {
+                fill_slice<THREADS>(g, n, verdict == FILL_NAN ? zn_nan() : 0.f);
+            }
+            __syncwarp();
+            if (lane == 0) zn_bar_arrive(&s.done[place]);
+            if (++place == ring) {
+                place = 0;
+                phase ^= 1;
+            }
+        }
     }
+    __syncwarp();
+    zn_cluster_arrive();         // a block's shared memory may be written by another one until both are here
+    zn_cluster_wait();
 }
 
-// Blocks per row and values of a slice kept on chip.  Three blocks share an SM while a slice has at most KEEP_3 values, so
-// that one loads while another stores; a vocabulary above 8 slices of that size gets larger ones, and what no longer fits
-// is read a second time.  Fewer rows than SMs are spread over more blocks, down to 2048 values each.
-constexpr int64_t KEEP_3 = 16640, KEEP_1 = 55000;
+// Blocks per row, values of a slice on chip, places in the ring, and threads.  A row is cut into as few slices as leave
+// room for three of them in a block, eight at most; larger vocabularies get a shorter ring, and what does not fit even
+// once is read a second time.  Where there are fewer rows than SMs they are spread over more blocks, down to 2048 values
+// each.
+constexpr size_t SMEM = 227 * 1024 - sizeof(Shared) - 64;
 struct Plan {
-    int share;
-    int64_t slice, keep;
+    int share, slice, keep, ring, threads;
+    size_t smem;
 };
-Plan distill_plan(int64_t rows, int64_t vocab, int sms) {
-    int share = 1;
-    while (share < MAX_SHARE && (vocab > share * KEEP_3 || (rows * share < 2 * sms && vocab > share * 2048))) share *= 2;
-    const int64_t slice = ((vocab + share - 1) / share + 3) / 4 * 4;
-    const int64_t keep = slice <= KEEP_1 ? slice : KEEP_1;
-    return {share, slice, keep};
+Plan distill_plan(int64_t rows, int64_t vocab, int64_t k, int sms) {
+    Plan p;
+    const auto smem = [&](int64_t keep, int ring) { return (size_t)ring * (size_t)(4 * (keep + 4) + 16 * k); };
+    const auto slice_of = [&](int share) { return ((vocab + share - 1) / share + 3) / 4 * 4; };
+    p.share = 1;
+    while (p.share < MAX_SHARE && (smem(slice_of(p.share), MAX_RING) > SMEM || (rows * p.share * 2 <= sms && slice_of(p.share) > 4096))) p.share *= 2;
+    p.slice = (int)slice_of(p.share);
+    p.ring = MAX_RING;
+    while (p.ring > 1 && smem(p.slice, p.ring) > SMEM) --p.ring;
+    p.keep = p.slice;
+    if (smem(p.keep, 1) > SMEM) p.keep = (int)((SMEM - 16 * k) / 4 - 8) / 4 * 4;
+    p.threads = 64;
+    while (p.threads < 512 && p.slice > p.threads * HELD) p.threads *= 2;
+    p.smem = smem(p.keep, p.ring);
+    return p;
+}
+
+template <int THREADS, bool REGS, bool WHOLE>
+zn_status launch(zn_ctx *ctx, const zn_distill_args &a, const Plan &p) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)p.share);
+    cfg.blockDim = dim3(THREADS + 64 + 32 * MAX_RING);
+    cfg.dynamicSmemBytes = p.smem;
+    cfg.stream = ctx->stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)p.share;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    // as many clusters as the GPU holds at once go from row to row
+    int &fit = ctx->cluster_fit[{(size_t)(4 * THREADS + 2 * REGS + WHOLE), (size_t)p.share, p.smem}];
+    if (fit == 0) {
+        ZN_CUDA(ctx, cudaFuncSetAttribute(distill_kernel<THREADS, REGS, WHOLE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SMEM));
+        ZN_CUDA(ctx, cudaOccupancyMaxActiveClusters(&fit, distill_kernel<THREADS, REGS, WHOLE>, &cfg));
+        if (fit < 1) fit = 1;
+    }
+    const int clusters = fit > a.rows ? (int)a.rows : fit;
+    cfg.gridDim = dim3((unsigned)(clusters * p.share));
+    zn_launch_scope scope(ctx, ZN_PROF_LOSS, 6.0 * a.rows * a.vocab, (a.grad ? 8.0 : 4.0) * a.rows * a.vocab);
+    ZN_CUDA(ctx, cudaLaunchKernelEx(&cfg, distill_kernel<THREADS, REGS, WHOLE>, a, p.share, p.slice, p.keep, p.ring, ctx->status_dev));
+    return ZN_OK;
 }
 
 }   // namespace
 
 zn_token_plan zn_plan_distill(size_t rows, size_t vocab, size_t k, int sms) {
-    (void)k;
-    const Plan d = distill_plan((int64_t)rows, (int64_t)vocab, sms);
+    const Plan d = distill_plan((int64_t)rows, (int64_t)vocab, (int64_t)k, sms);
     zn_token_plan p;
-    p.threads = TPB;
+    p.threads = d.threads + 64 + 32 * MAX_RING;
     p.share = d.share;
-    p.blocks = (int64_t)rows * d.share;
-    p.smem = (size_t)(d.keep + 4) * sizeof(float);
+    p.blocks = (rows < (size_t)sms ? (int64_t)rows : sms) * d.share;       // at most; the launch asks how many fit at once
+    p.smem = d.smem;
     return p;
 }
 
 zn_status zn_k_distill(zn_ctx *ctx, const zn_distill_args &a) {
-    const Plan d = distill_plan(a.rows, a.vocab, ctx->sm_count);
-    const zn_token_plan p = zn_plan_distill((size_t)a.rows, (size_t)a.vocab, (size_t)a.k, ctx->sm_count);
-    ZN_CUDA(ctx, cudaFuncSetAttribute(distill_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)((KEEP_1 + 4) * sizeof(float))));
-    zn_launch_scope scope(ctx, ZN_PROF_LOSS, 6.0 * a.rows * a.vocab, (a.grad ? 8.0 : 4.0) * a.rows * a.vocab);
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)p.blocks);
-    cfg.blockDim = dim3(p.threads);
-    cfg.dynamicSmemBytes = p.smem;
-    cfg.stream = ctx->stream;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = (unsigned)d.share;
-    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    ZN_CUDA(ctx, cudaLaunchKernelEx(&cfg, distill_kernel, a, d.share, d.slice, d.keep, ctx->status_dev));
-    return ZN_OK;
+    const Plan p = distill_plan(a.rows, a.vocab, a.k, ctx->sm_count);
+    if (p.keep < p.slice) return launch<512, false, false>(ctx, a, p);
+    if (p.slice > p.threads * HELD) return launch<512, false, true>(ctx, a, p);
+    switch (p.threads) {
+    case 512: return launch<512, true, true>(ctx, a, p);
+    case 256: return launch<256, true, true>(ctx, a, p);
+    case 128: return launch<128, true, true>(ctx, a, p);
+    default: return launch<64, true, true>(ctx, a, p);
+    }
 }

@@ -163,7 +163,7 @@ __global__ void __launch_bounds__(TPB, 4) scores_kernel(zn_scores_args a, int pi
             offer(list, key, k);
         }
     }
-    st = zn_softmax_block<TPB>(st, c, part);
+    st = zn_softmax_block<TPB, true>(st, c, part, [] { __syncthreads(); });
     if (k > 0) cut_list(list, k);
     int kept = list.count;
     if (pieces > 1) {
@@ -194,13 +194,10 @@ __global__ void __launch_bounds__(TPB, 4) scores_kernel(zn_scores_args a, int pi
             if (k > 0) list.key[threadIdx.x] = __ldcg(reinterpret_cast<const unsigned long long *>(rec + 4) + share);
         }
         __syncthreads();
-        st = piece_stats[0];
+        st = zn_softmax_join<true>(pieces, c, [&](int i) { return piece_stats[i]; });
+        // every piece has share + 1 keys at or above the lowest of these, so k in all
         unsigned long long bar = list.key[0];
-        for (int p = 1; p < pieces; ++p) {
-            zn_softmax_join(st, piece_stats[p], c);
-            // every piece has share + 1 keys at or above the lowest of these, so k in all
-            bar = min(bar, list.key[p]);
-        }
+        for (int p = 1; p < pieces; ++p) bar = min(bar, list.key[p]);
         __syncthreads();
         if (k > 0) {
             if (threadIdx.x == 0 && bar != 0) list.bar = bar - 1;

@@ -6,8 +6,10 @@
 #include <cstdlib>
 #include <cuda_bf16.h>
 
+#include <array>
 #include <cstdint>
 #include <cstdio>
+#include <map>
 #include <string>
 #include <unordered_map>
 #include <vector>
@@ -79,6 +81,9 @@ struct zn_ctx {
     // Arrival counters of the reductions that finish in their own last block (column sums, sums of squares, loss
     // sums): 1024 per lane, all zero between launches (the block that finishes a reduction clears what it used).
     unsigned int *block_counters = nullptr;
+
+    // Clusters of the distillation kernel that the GPU holds at once, by threads, blocks per cluster and shared memory.
+    std::map<std::array<size_t, 3>, int> cluster_fit;
 
     zn_dp_state *dp = nullptr;
 };
