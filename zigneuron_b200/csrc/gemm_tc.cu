@@ -1179,6 +1179,12 @@ struct TmapKey {
     int es, box_inner, box_outer, swizzle;
 };
 
+}   // namespace
+
+void *zn_tensor_map_encoder() { return reinterpret_cast<void *>(get_encode()); }
+
+namespace {
+
 zn_status make_tmap(zn_ctx *ctx, CUtensorMap *out, int es, const void *ptr, int64_t inner, int64_t outer, int64_t ld,
                     int box_inner, int box_outer, int swizzle_kind) {
     TmapKey k;

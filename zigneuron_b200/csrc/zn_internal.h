@@ -189,6 +189,8 @@ zn_status zn_gemm_simt(zn_ctx *ctx, const float *a, int64_t a_rs, int64_t a_cs, 
 zn_status zn_gemm_tc(zn_ctx *ctx, int elem_type, const void *a, int64_t lda, bool a_mn_major, const void *b,
                      int64_t ldb, bool b_mn_major, int64_t m, int64_t n, int64_t k, const zn_epilogue &ep);
 
+void *zn_tensor_map_encoder();         // cuTensorMapEncodeTiled of the driver, or null
+
 // Row-major helpers.  T = float or __nv_bfloat16 selected by is_bf16.
 zn_status zn_k_convert(zn_ctx *ctx, const float *src, int64_t ld_src, void *dst, int64_t ld_dst, bool dst_bf16,
                        int64_t rows, int64_t cols);   // pads columns [cols, ld_dst) with zeros

@@ -181,6 +181,13 @@ __device__ __forceinline__ void zn_bulk_load(void *dst, const void *src, uint32_
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
                  ::"r"(zn_smem(dst)), "l"(src), "r"(bytes), "r"(zn_smem(bar)) : "memory");
 }
+// Four bytes in the background, zero where there are none; this thread's arrival on `bar` once all it asked for is there.
+__device__ __forceinline__ void zn_async_word(void *dst, const void *src, bool there) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(zn_smem(dst)), "l"(src), "r"(there ? 4 : 0) : "memory");
+}
+__device__ __forceinline__ void zn_async_words_arrive(uint64_t *bar) {
+    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(zn_smem(bar)) : "memory");
+}
 __device__ __forceinline__ void zn_cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
 __device__ __forceinline__ void zn_cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 // Two floats to the same place in block `rank` of the cluster; they count 8 bytes on that block's `bar`.
