@@ -256,19 +256,19 @@ __global__ void __launch_bounds__(THREADS + 64 + 32 * MAX_RING) distill_kernel(z
                         const float4 f = *reinterpret_cast<const float4 *>(mine + from + 4 * (i + j * THREADS));
                         u[4 * j] = f.x; u[4 * j + 1] = f.y; u[4 * j + 2] = f.z; u[4 * j + 3] = f.w;
                     }
-                    zn_softmax_add<16, false>(st, u, c);
+                    zn_softmax_add<16, false>(st, u, zn_largest(u), c);
                 }
                 for (; i < vecs; i += THREADS) {
                     const float4 f = *reinterpret_cast<const float4 *>(mine + from + 4 * i);
                     const float u[4] = {f.x, f.y, f.z, f.w};
-                    zn_softmax_add<4, false>(st, u, c);
+                    zn_softmax_add<4, false>(st, u, zn_largest(u), c);
                 }
                 const float u[1] = {end};
-                zn_softmax_add<1, false>(st, u, c);
+                zn_softmax_add<1, false>(st, u, u[0], c);
                 if (!WHOLE)         // up to four of them are in `ends` already
                     for (int j = on_chip + 4 + threadIdx.x; j < n; j += THREADS) {
                         const float o[1] = {x[j]};
-                        zn_softmax_add<1, false>(st, o, c);
+                        zn_softmax_add<1, false>(st, o, o[0], c);
                     }
             }
             // over the warp, then over all warps of the row's blocks: each sends what it has to every block

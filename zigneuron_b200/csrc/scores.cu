@@ -14,9 +14,9 @@ __device__ __forceinline__ unsigned long long rank_key(float x, int64_t c) {
     return x == -INFINITY ? 0ull : ((unsigned long long)u << 32) | (uint32_t)(0xffffffffu - (uint32_t)c);
 }
 
-// The k largest keys seen by a block.  Keys above the bar go into a list; when it is nearly full it is sorted and
-// cut to k, and the bar rises to the k-th.  The result does not depend on the order in which keys arrive: keys are
-// distinct.  `count` and `bar` are read by all threads between barriers only.
+// The k largest keys seen by a block.  Keys above the bar go into a list; when it is half full it is sorted and cut to k,
+// and the bar rises to the k-th.  The result does not depend on the order in which keys arrive: keys are distinct.
+// `count` and `bar` are read by all threads between barriers only.
 constexpr int LIST = 1024;
 struct TopList {
     unsigned long long key[LIST];
@@ -24,9 +24,23 @@ struct TopList {
     int count;
 };
 
-// Sorts the first n keys, largest first (bitonic network over the next power of two, filled up with zeros).
+// Sorts the first n keys, largest first: a short list by counting, for each key, those above it; a long one by a bitonic
+// network over the next power of two, filled up with zeros.
 __device__ void sort_list(TopList &t, int n) {
-    int size = 32;
+    __syncthreads();
+    if (n <= TPB) {
+        const unsigned long long mine = threadIdx.x < n ? t.key[threadIdx.x] : 0ull;
+        int place = 0;
+        if (threadIdx.x < n) {
+#pragma unroll 4
+            for (int i = 0; i < n; ++i) place += t.key[i] > mine;
+        }
+        __syncthreads();
+        if (threadIdx.x < n) t.key[place] = mine;
+        __syncthreads();
+        return;
+    }
+    int size = 2 * TPB;
     while (size < n) size *= 2;
     for (int i = n + threadIdx.x; i < size; i += TPB) t.key[i] = 0;
     for (int run = 2; run <= size; run *= 2)
@@ -52,35 +66,44 @@ __device__ void cut_list(TopList &t, int k) {
     __syncthreads();
 }
 
-// Offers one tile of keys, N per thread (0 = none).  Usually all that reach the bar fit behind the list; where they do not
-// (a sorted row, say), the tile is taken back and offered again in steps that always fit.
-template <int N>
-__device__ void offer(TopList &t, const unsigned long long (&key)[N], int k) {
-    const int before = t.count;
-    const unsigned long long bar = t.bar;
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < N; ++i)
-        if (key[i] > bar) {
-            const int at = atomicAdd(&t.count, 1);
-            if (at < LIST) t.key[at] = key[i];
-        }
-    __syncthreads();
-    if (t.count <= LIST) {
-        if (t.count > LIST / 2) cut_list(t, k);
-        return;
+// Puts a key above the bar on the list, if it has room; returns how full the list is.
+__device__ __forceinline__ int put_key(TopList &t, unsigned long long key, unsigned long long bar) {
+    if (key <= bar) return 0;
+    const int at = atomicAdd(&t.count, 1);
+    if (at < LIST) t.key[at] = key;
+    return at;
+}
+
+// After every thread has put its keys: cuts a list that is half full; true if the bar has risen.  Where not all had room (a
+// sorted row, say) what is on the list is cut, and the tile's keys are put again in steps that always fit, but for those
+// that are on it already.
+template <int N, typename F>
+__device__ __forceinline__ bool settle(TopList &t, int k, int fullest, bool cut, F key) {
+    if (!__syncthreads_or(fullest >= LIST / 2)) {
+        if (cut) cut_list(t, k);
+        return cut;
     }
+    const bool again = __syncthreads_or(fullest >= LIST);
+    if (again && threadIdx.x == 0) t.count = LIST;
     __syncthreads();
-    if (threadIdx.x == 0) t.count = before;
-    __syncthreads();
-#pragma unroll
+    cut_list(t, k);
+    if (!again) return true;
+    int kept = t.count;
+#pragma unroll 1
     for (int i = 0; i < N; ++i) {
-        if (t.count > LIST - TPB) cut_list(t, k);
-        const unsigned long long now = t.bar;
+        if (t.count > LIST - TPB) {
+            cut_list(t, k);
+            kept = t.count;
+        }
+        const unsigned long long bar = t.bar, mine = key(i);
+        bool there = mine <= bar;
+        for (int j = 0; j < kept && !there; ++j) there = t.key[j] == mine;
         __syncthreads();
-        if (key[i] > now) t.key[atomicAdd(&t.count, 1)] = key[i];
+        if (!there) put_key(t, mine, bar);
         __syncthreads();
     }
+    cut_list(t, k);
+    return true;
 }
 
 // One row, or one piece of it where rows alone would leave SMs idle (then the block that finishes a row last joins the
@@ -89,7 +112,7 @@ __device__ void offer(TopList &t, const unsigned long long (&key)[N], int k) {
 constexpr int TILE = TPB * 16;
 constexpr int MAX_PIECES = 64;
 
-__global__ void __launch_bounds__(TPB, 4) scores_kernel(zn_scores_args a, int pieces, int64_t piece_len, float *scratch, unsigned int *arrivals,
+__global__ void __launch_bounds__(TPB, 3) scores_kernel(zn_scores_args a, int pieces, int64_t piece_len, float *scratch, unsigned int *arrivals,
                                                         int *status) {
     __shared__ zn_softmax part[TPB / 32];
     __shared__ TopList list;
@@ -98,7 +121,7 @@ __global__ void __launch_bounds__(TPB, 4) scores_kernel(zn_scores_args a, int pi
     const int64_t r = blockIdx.x / pieces;
     const int piece = (int)(blockIdx.x % pieces);
     const float *x = a.logits + r * a.ld;
-    const int64_t lo = piece * piece_len, hi = min(a.vocab, lo + piece_len);
+    const int lo = (int)(piece * piece_len), hi = (int)min(a.vocab, lo + piece_len);
     const float c = 1.4426950408889634f / a.temperature;
     const int k = a.top_k;
     zn_softmax st{-INFINITY, 0.f, 0.f};
@@ -107,61 +130,81 @@ __global__ void __launch_bounds__(TPB, 4) scores_kernel(zn_scores_args a, int pi
         list.bar = 0;
     }
     __syncthreads();
-    bool first = true;
-    // the tile that holds the unaligned ends of the piece comes on top of the aligned ones
-    const int64_t from = lo + zn_aligned_from(x + lo, hi - lo), vecs = (hi - from) / 4, to = from + 4 * vecs;
-    const int64_t tiles = (vecs + TPB * 4 - 1) / (TPB * 4);
-    for (int64_t t = 0; t <= tiles; ++t) {
+    const int from = lo + (int)zn_aligned_from(x + lo, hi - lo), vecs = (hi - from) / 4, to = from + 4 * vecs;
+    {
+        // up to six values around the aligned part
+        const int at = threadIdx.x < 4 ? lo + threadIdx.x : to + threadIdx.x - 4;
+        const bool there = threadIdx.x < 8 && (threadIdx.x < 4 ? at < from : at < hi);
+        const float v[1] = {there ? x[at] : -INFINITY};
+        zn_softmax_add<1, true>(st, v, v[0], c);
+        if (k > 0 && v[0] > -INFINITY) put_key(list, rank_key(v[0], at), 0ull);
+    }
+    unsigned long long bar = 0;
+    float bar_x = -INFINITY;
+    const auto read_bar = [&]() {
+        bar = list.bar;
+        const uint32_t u = (uint32_t)(bar >> 32);
+        bar_x = bar == 0 ? -INFINITY : __uint_as_float((u & 0x80000000u) ? u & 0x7fffffffu : ~u);
+    };
+    const float4 *p = reinterpret_cast<const float4 *>(x + from) + threadIdx.x;
+    const float4 none = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+    float4 next[4];                      // the tile after this one is on its way
+#pragma unroll
+    for (int j = 0; j < 4; ++j) next[j] = j * TPB + (int)threadIdx.x < vecs ? __ldcs(p + j * TPB) : none;
+    for (int v0 = 0; v0 < vecs; v0 += TPB * 4) {
         float v[16];
-        int64_t at[4];
-        if (t < tiles) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int64_t i = (t * 4 + j) * TPB + threadIdx.x;
-                at[j] = from + 4 * i;
-                float4 f = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
-                if (i < vecs) f = __ldcs(reinterpret_cast<const float4 *>(x + at[j]));
-                v[4 * j] = f.x; v[4 * j + 1] = f.y; v[4 * j + 2] = f.z; v[4 * j + 3] = f.w;
-            }
-        } else {
-            if (from == lo && to == hi) break;
-#pragma unroll
-            for (int i = 0; i < 16; ++i) v[i] = -INFINITY;
-            const int64_t i = threadIdx.x < 4 ? lo + threadIdx.x : to + (threadIdx.x - 4);
-            at[0] = i;
-            at[1] = at[2] = at[3] = 0;
-            if (threadIdx.x < 8 && (threadIdx.x < 4 ? i < from : i < hi)) v[0] = x[i];
+        for (int j = 0; j < 4; ++j) {
+            v[4 * j] = next[j].x; v[4 * j + 1] = next[j].y; v[4 * j + 2] = next[j].z; v[4 * j + 3] = next[j].w;
+            const int i = v0 + (4 + j) * TPB;
+            next[j] = i + (int)threadIdx.x < vecs ? __ldcs(p + i) : none;
         }
-        zn_softmax_add<16, true>(st, v, c);
+        float top = zn_largest(v);
+        zn_softmax_add<16, true>(st, v, top, c);
         if (k == 0) continue;
-        unsigned long long bar = list.bar;
-        if (first) {
-            // the k-th largest of the threads' own largest is a bar that at least k values reach
-            unsigned long long mine = 0;
+        const int col0 = from + 4 * (v0 + (int)threadIdx.x);
+        const auto key_of = [&](int i) {
+            float u = v[0];
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const unsigned long long o = rank_key(v[i], at[i / 4] + i % 4);
-                if (v[i] > -INFINITY && o > mine) mine = o;
+            for (int j = 1; j < 16; ++j) u = i == j ? v[j] : u;
+            return u > -INFINITY ? rank_key(u, col0 + i / 4 * (4 * TPB) + i % 4) : 0ull;
+        };
+        if (v0 == 0) {
+            // A bar for the first tile: threads stand in groups, at least k of them.  Each group's largest value reaches
+            // the lowest of these, so at least k values do.
+            float mine = top;
+            int width = 32;
+            while (width > 2 && TPB / width < k) width /= 2;
+            for (int o = width / 2; o > 0; o /= 2) mine = fmaxf(mine, __shfl_xor_sync(0xffffffffu, mine, o));
+            const bool some = mine > -INFINITY;
+            const int groups = __popc(__ballot_sync(0xffffffffu, some)) / width;
+            const float low = -zn_warp_max(some ? -mine : -INFINITY);
+            if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = {low, (float)groups, 0.f};
+            __syncthreads();
+            if (threadIdx.x == 0) {
+                float lowest = INFINITY;
+                int all = 0;
+                for (int w = 0; w < TPB / 32; ++w) {
+                    lowest = fminf(lowest, part[w].m);
+                    all += (int)part[w].s;
+                }
+                if (all >= k) list.bar = rank_key(lowest, 0xffffffffll);
             }
-            list.key[threadIdx.x] = mine;
             __syncthreads();
-            sort_list(list, TPB);
-            if (threadIdx.x == 0 && list.key[k - 1] != 0) list.bar = list.key[k - 1] - 1;
-            __syncthreads();
-            bar = list.bar;
-            first = false;
+            read_bar();
         }
-        const uint32_t bar_value = (uint32_t)(bar >> 32);
-        const float bar_x = bar == 0 ? -INFINITY : __uint_as_float((bar_value & 0x80000000u) ? bar_value & 0x7fffffffu : ~bar_value);
-        unsigned long long key[16];
-        bool any = false;
+        int fullest = 0;
+        if (top >= bar_x) {
+            uint32_t reach = 0;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) any = any || v[i] >= bar_x;
-        if (__syncthreads_or(any)) {
-#pragma unroll
-            for (int i = 0; i < 16; ++i) key[i] = v[i] > -INFINITY ? rank_key(v[i], at[i / 4] + i % 4) : 0ull;
-            offer(list, key, k);
+            for (int i = 0; i < 16; ++i) reach |= v[i] >= bar_x ? 1u << i : 0u;
+            while (reach) {
+                const int i = __ffs(reach) - 1;
+                reach &= reach - 1;
+                fullest = max(fullest, put_key(list, key_of(i), bar));
+            }
         }
+        if (settle<16>(list, k, fullest, v0 == 0, key_of)) read_bar();
     }
     st = zn_softmax_block<TPB, true>(st, c, part, [] { __syncthreads(); });
     if (k > 0) cut_list(list, k);
@@ -196,22 +239,25 @@ __global__ void __launch_bounds__(TPB, 4) scores_kernel(zn_scores_args a, int pi
         __syncthreads();
         st = zn_softmax_join<true>(pieces, c, [&](int i) { return piece_stats[i]; });
         // every piece has share + 1 keys at or above the lowest of these, so k in all
-        unsigned long long bar = list.key[0];
-        for (int p = 1; p < pieces; ++p) bar = min(bar, list.key[p]);
+        bar = list.key[0];
+        for (int i = 1; i < pieces; ++i) bar = min(bar, list.key[i]);
         __syncthreads();
         if (k > 0) {
             if (threadIdx.x == 0 && bar != 0) list.bar = bar - 1;
             __syncthreads();
-            for (int64_t i0 = 0; i0 < (int64_t)pieces * k; i0 += TPB * 4) {
+            for (int i0 = 0; i0 < pieces * k; i0 += TPB * 4) {
                 unsigned long long key[4];
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    const int64_t i = i0 + j * TPB + threadIdx.x;
-                    key[j] = i < (int64_t)pieces * k
-                                 ? __ldcg(reinterpret_cast<const unsigned long long *>(scratch + (r * pieces + i / k) * record + 4) + i % k)
-                                 : 0ull;
+                    const int i = i0 + j * TPB + threadIdx.x;
+                    key[j] = i < pieces * k ? __ldcg(reinterpret_cast<const unsigned long long *>(scratch + (r * pieces + i / k) * record + 4) + i % k) : 0ull;
                 }
-                offer(list, key, k);
+                bar = list.bar;
+                __syncthreads();
+                int fullest = 0;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) fullest = max(fullest, put_key(list, key[j], bar));
+                settle<4>(list, k, fullest, false, [&](int i) { return i == 0 ? key[0] : i == 1 ? key[1] : i == 2 ? key[2] : key[3]; });
             }
             cut_list(list, k);
             kept = list.count;
@@ -224,7 +270,7 @@ __global__ void __launch_bounds__(TPB, 4) scores_kernel(zn_scores_args a, int pi
             a.stats[2 * r] = bad ? nan : st.m;
             a.stats[2 * r + 1] = bad ? nan : empty ? -INFINITY : ls;
         }
-        if (a.entropy) a.entropy[r] = bad ? nan : empty ? 0.f : ls - st.w * inv_t / st.s;
+        if (a.entropy) a.entropy[r] = bad ? nan : empty ? 0.f : ls - st.w * 0.6931471805599453f / st.s;
         if (a.logprob) {
             const int64_t t = a.tokens[r];
             float lp = 0.f;

@@ -49,43 +49,44 @@ __device__ __forceinline__ float zn_exp2(float v) {
 }
 __device__ __forceinline__ float zn_nan() { return __int_as_float(0x7fffffff); }
 
-// Softmax statistics kept on the way over a row: with m the largest logit so far, s = sum 2^((x - m) c) and
-// w = sum 2^((x - m) c) (x - m), where c = log2(e) / T.  The difference is formed before the scaling: a product x c could
-// leave the range of float where x - m does not.  A column at -inf adds nothing to either; a NaN or +inf makes s NaN.
+// Softmax statistics kept on the way over a row: with m the largest logit so far, c = log2(e) / T and y = (x - m) c,
+// s = sum 2^y and w = sum 2^y y.  The difference is formed before the scaling: a product x c could leave the range of float
+// where x - m does not.  A column at -inf adds nothing to either; a NaN or +inf makes s NaN.
 struct zn_softmax {
     float m, s, w;
 };
-// A difference so low that its term is zero, kept finite: zero times -inf would be NaN (and 2^31 of these still fit).
-__device__ __forceinline__ float zn_above(float d) { return fmaxf(d, -1e28f); }
-// N values at once, with one change of the maximum at most.
-template <int N, bool ENTROPY>
-__device__ __forceinline__ void zn_softmax_add(zn_softmax &a, const float (&x)[N], float c) {
-    float top = x[0];
-#pragma unroll
-    for (int i = 1; i < N; ++i) top = fmaxf(top, x[i]);
-    if (top > a.m) {
-        if (a.m > -INFINITY) {
-            const float d = a.m - top, f = zn_exp2(d * c);
-            if (ENTROPY) a.w = f * (a.w + a.s * zn_above(d));
-            a.s *= f;
-        }
-        a.m = top;
-    }
-    const float base = a.m == -INFINITY ? 0.f : a.m;
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-        const float d = x[i] - base, e = zn_exp2(d * c);
-        a.s += e;
-        if (ENTROPY) a.w = fmaf(e, zn_above(d), a.w);
-    }
+// An exponent so low that its power is zero, kept finite (zero times -inf would be NaN); NaN stays NaN.
+__device__ __forceinline__ float zn_exponent(float y) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(y), "f"(-200.f));
+    return r;
 }
 // The statistics brought to a larger maximum m.
 template <bool ENTROPY>
 __device__ __forceinline__ void zn_softmax_raise(zn_softmax &a, float m, float c) {
-    const float d = a.m == m ? 0.f : a.m - m, f = zn_exp2(d * c);       // both at -inf: no difference
-    if (ENTROPY) a.w = f * (a.w + a.s * zn_above(d));
+    const float y = a.m == m ? 0.f : zn_exponent((a.m - m) * c), f = zn_exp2(y);       // both at -inf: no difference
+    if (ENTROPY) a.w = f * (a.w + a.s * y);
     a.s *= f;
     a.m = m;
+}
+// N values at once, `top` the largest, with one change of the maximum at most.
+template <int N>
+__device__ __forceinline__ float zn_largest(const float (&x)[N]) {
+    float top = x[0];
+#pragma unroll
+    for (int i = 1; i < N; ++i) top = fmaxf(top, x[i]);
+    return top;
+}
+template <int N, bool ENTROPY>
+__device__ __forceinline__ void zn_softmax_add(zn_softmax &a, const float (&x)[N], float top, float c) {
+    if (top > a.m) zn_softmax_raise<ENTROPY>(a, top, c);
+    const float base = a.m == -INFINITY ? 0.f : a.m;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const float y = ENTROPY ? zn_exponent((x[i] - base) * c) : (x[i] - base) * c, e = zn_exp2(y);
+        a.s += e;
+        if (ENTROPY) a.w = fmaf(e, y, a.w);
+    }
 }
 // Over the first THREADS threads of a block, all of which get the same result: first the maximum, then the sums, which
 // takes one exponential per thread.  `sync` is a barrier among them; `part` holds one entry per warp.
