@@ -188,7 +188,7 @@ def check_scores(got, want, k):
 
 SCORES = [(1, 1, 1, 1.0, 1), (1, 5, 5, 2.0, 8), (3, 17, 20, 0.7, 17), (2, 129, 129, 1.0, 128), (5, 1000, 1003, 1.3, 3), (300, 999, 999, 1.0, 10),
           (1, 131072, 131072, 0.8, 20), (7, 50001, 50001, 1.0, 128), (2, 200003, 200010, 3.0, 64), (700, 4099, 4100, 1.0, 5),
-          (1500, 257, 260, 0.5, 40), (64, 32768, 32768, 1.0, 0), (640, 20001, 20001, 1.0, 31), (13, 8191, 8192, 1.0, 1)]
+          (1500, 257, 260, 0.5, 40), (900, 3000, 3001, 1.0, 100), (600, 1025, 1027, 1.0, 64), (600, 2048, 2048, 0.9, 128), (3, 8000, 8000, 1.0, 65), (64, 32768, 32768, 1.0, 0), (640, 20001, 20001, 1.0, 31), (13, 8191, 8192, 1.0, 1)]
 
 
 @pytest.mark.parametrize("rows,vocab,ld,t,k", SCORES)
@@ -551,7 +551,7 @@ def test_quantize4(be, n, k, group):
 
 
 MATMUL4 = [(1, 1, 1, 32), (1, 7, 5, 64), (1, 64, 128, 128), (1, 4096, 4096, 64), (2, 100, 257, 32), (3, 1003, 640, 64), (8, 333, 1000, 128),
-           (5, 17, 4000, 32), (16, 129, 513, 64), (17, 64, 300, 32), (40, 200, 1025, 128), (1, 20001, 512, 128), (7, 50, 8192, 128), (1, 31, 30000, 64)]
+           (5, 17, 4000, 32), (16, 129, 513, 64), (17, 64, 300, 32), (2, 12000, 2000, 64), (9, 10001, 1100, 32), (6, 19300, 4100, 128), (40, 200, 1025, 128), (1, 20001, 512, 128), (7, 50, 8192, 128), (1, 31, 30000, 64)]
 
 
 @pytest.mark.parametrize("act", ["linear", "relu", "gelu"])

@@ -4,7 +4,7 @@
 
 namespace {
 
-constexpr int TPB = 256;
+constexpr int GRAD_TPB = 256;
 
 // A logit and its column as one number that orders by value, then by lowest column: larger is better.  0 is "none".
 __device__ __forceinline__ unsigned long long rank_key(float x, int64_t c) {
@@ -26,13 +26,14 @@ struct TopList {
 
 // Sorts the first n keys, largest first: a short list by counting, for each key, those above it; a long one by a bitonic
 // network over the next power of two, filled up with zeros.
+template <int TPB>
 __device__ void sort_list(TopList &t, int n) {
     __syncthreads();
     if (n <= TPB) {
         const unsigned long long mine = threadIdx.x < n ? t.key[threadIdx.x] : 0ull;
         int place = 0;
         if (threadIdx.x < n) {
-#pragma unroll 4
+#pragma unroll 8
             for (int i = 0; i < n; ++i) place += t.key[i] > mine;
         }
         __syncthreads();
@@ -56,9 +57,10 @@ __device__ void sort_list(TopList &t, int n) {
 }
 
 // Cuts the list to its k largest keys, sorted.
+template <int TPB>
 __device__ void cut_list(TopList &t, int k) {
     const int n = t.count;
-    sort_list(t, n);
+    sort_list<TPB>(t, n);
     if (threadIdx.x == 0) {
         t.count = n < k ? n : k;
         if (n >= k) t.bar = t.key[k - 1];
@@ -66,56 +68,37 @@ __device__ void cut_list(TopList &t, int k) {
     __syncthreads();
 }
 
-// Puts a key above the bar on the list, if it has room; returns how full the list is.
-__device__ __forceinline__ int put_key(TopList &t, unsigned long long key, unsigned long long bar) {
-    if (key <= bar) return 0;
+// Puts a key above the bar on the list, if it has room; the count goes on where it has not.
+__device__ __forceinline__ void put_key(TopList &t, unsigned long long key, unsigned long long bar) {
+    if (key <= bar) return;
     const int at = atomicAdd(&t.count, 1);
     if (at < LIST) t.key[at] = key;
-    return at;
 }
 
-// After every thread has put its keys: cuts a list that is half full; true if the bar has risen.  Where not all had room (a
-// sorted row, say) what is on the list is cut, and the tile's keys are put again in steps that always fit, but for those
-// that are on it already.
-template <int N, typename F>
-__device__ __forceinline__ bool settle(TopList &t, int k, int fullest, bool cut, F key) {
-    if (!__syncthreads_or(fullest >= LIST / 2)) {
-        if (cut) cut_list(t, k);
-        return cut;
-    }
-    const bool again = __syncthreads_or(fullest >= LIST);
-    if (again && threadIdx.x == 0) t.count = LIST;
+// One step of the slow way, taken where a list has run over (a sorted row, say): at most one key a thread, and the list is
+// cut whenever another step might not fit.
+template <int TPB>
+__device__ __forceinline__ void put_step(TopList &t, int k, unsigned long long key) {
+    if (t.count > LIST - TPB) cut_list<TPB>(t, k);
+    const unsigned long long bar = t.bar;
     __syncthreads();
-    cut_list(t, k);
-    if (!again) return true;
-    int kept = t.count;
-#pragma unroll 1
-    for (int i = 0; i < N; ++i) {
-        if (t.count > LIST - TPB) {
-            cut_list(t, k);
-            kept = t.count;
-        }
-        const unsigned long long bar = t.bar, mine = key(i);
-        bool there = mine <= bar;
-        for (int j = 0; j < kept && !there; ++j) there = t.key[j] == mine;
-        __syncthreads();
-        if (!there) put_key(t, mine, bar);
-        __syncthreads();
-    }
-    cut_list(t, k);
-    return true;
+    put_key(t, key, bar);
+    __syncthreads();
 }
 
 // One row, or one piece of it where rows alone would leave SMs idle (then the block that finishes a row last joins the
 // pieces, in their order).  The row is read once: 16 values a thread at a time, as 16-byte loads from the first aligned
-// one on; the statistics stay in registers and the few values that reach the bar go to the list.
-constexpr int TILE = TPB * 16;
+// one on; the statistics stay in registers and the few values that reach the bar go to the list.  The list is looked after
+// when the number of tiles has doubled, not tile by tile: about k values pass the bar in between, and barriers are what
+// such a loop can least afford.
 constexpr int MAX_PIECES = 64;
 
-__global__ void __launch_bounds__(TPB, 3) scores_kernel(zn_scores_args a, int pieces, int64_t piece_len, float *scratch, unsigned int *arrivals,
+template <int TPB>
+__global__ void __launch_bounds__(TPB, 768 / TPB) scores_kernel(zn_scores_args a, int pieces, int64_t piece_len, float *scratch, unsigned int *arrivals,
                                                         int *status) {
     __shared__ zn_softmax part[TPB / 32];
     __shared__ TopList list;
+    __shared__ __align__(16) float largest[TPB];
     __shared__ zn_softmax piece_stats[MAX_PIECES];
     __shared__ bool last;
     const int64_t r = blockIdx.x / pieces;
@@ -148,6 +131,7 @@ __global__ void __launch_bounds__(TPB, 3) scores_kernel(zn_scores_args a, int pi
     };
     const float4 *p = reinterpret_cast<const float4 *>(x + from) + threadIdx.x;
     const float4 none = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+    int held = 0, since = 0, check = 0;  // the list's length at the last look, the first tile after it, the end of the next
     float4 next[4];                      // the tile after this one is on its way
 #pragma unroll
     for (int j = 0; j < 4; ++j) next[j] = j * TPB + (int)threadIdx.x < vecs ? __ldcs(p + j * TPB) : none;
@@ -159,55 +143,94 @@ __global__ void __launch_bounds__(TPB, 3) scores_kernel(zn_scores_args a, int pi
             const int i = v0 + (4 + j) * TPB;
             next[j] = i + (int)threadIdx.x < vecs ? __ldcs(p + i) : none;
         }
-        float top = zn_largest(v);
+        const float top = zn_largest(v);
         zn_softmax_add<16, true>(st, v, top, c);
         if (k == 0) continue;
-        const int col0 = from + 4 * (v0 + (int)threadIdx.x);
-        const auto key_of = [&](int i) {
+        const auto key_of = [&](const float (&v)[16], int v0, int i) {
             float u = v[0];
 #pragma unroll
             for (int j = 1; j < 16; ++j) u = i == j ? v[j] : u;
-            return u > -INFINITY ? rank_key(u, col0 + i / 4 * (4 * TPB) + i % 4) : 0ull;
+            return u > -INFINITY ? rank_key(u, from + 4 * (v0 + (int)threadIdx.x) + i / 4 * (4 * TPB) + i % 4) : 0ull;
         };
         if (v0 == 0) {
-            // A bar for the first tile: threads stand in groups, at least k of them.  Each group's largest value reaches
-            // the lowest of these, so at least k values do.
+            // A bar for the first tile: the k-th largest of the largest values of groups of threads, four to a group or (for
+            // a large k) each by itself.  At least k values reach it, and few more do.
+            const int width = k <= TPB / 8 ? 4 : 1, groups = TPB / width;
             float mine = top;
-            int width = 32;
-            while (width > 2 && TPB / width < k) width /= 2;
             for (int o = width / 2; o > 0; o /= 2) mine = fmaxf(mine, __shfl_xor_sync(0xffffffffu, mine, o));
-            const bool some = mine > -INFINITY;
-            const int groups = __popc(__ballot_sync(0xffffffffu, some)) / width;
-            const float low = -zn_warp_max(some ? -mine : -INFINITY);
-            if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = {low, (float)groups, 0.f};
+            if (threadIdx.x % width == 0) largest[threadIdx.x / width] = mine;
+            held = list.count;                       // the values around the aligned part
             __syncthreads();
-            if (threadIdx.x == 0) {
-                float lowest = INFINITY;
-                int all = 0;
-                for (int w = 0; w < TPB / 32; ++w) {
-                    lowest = fminf(lowest, part[w].m);
-                    all += (int)part[w].s;
+            if (threadIdx.x < groups) {
+                mine = largest[threadIdx.x];
+                int above = 0, reach = 0;
+                for (int i = 0; i < groups; i += 4) {
+                    const float4 f = *reinterpret_cast<const float4 *>(largest + i);
+                    above += (f.x > mine) + (f.y > mine) + (f.z > mine) + (f.w > mine);
+                    reach += (f.x >= mine) + (f.y >= mine) + (f.z >= mine) + (f.w >= mine);
                 }
-                if (all >= k) list.bar = rank_key(lowest, 0xffffffffll);
+                // equal ones write the same; below k values in all, nothing is barred
+                if (above < k && k <= reach && mine > -INFINITY) list.bar = rank_key(mine, 0xffffffffll);
             }
             __syncthreads();
             read_bar();
         }
-        int fullest = 0;
-        if (top >= bar_x) {
+        const int col0 = from + 4 * (v0 + (int)threadIdx.x);
+        if (v0 > 0) {
+            if (top >= bar_x) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    if (v[i] >= bar_x && v[i] > -INFINITY) put_key(list, rank_key(v[i], col0 + i / 4 * (4 * TPB) + i % 4), bar);
+            }
+        } else {
+            // most of the first tile's come at once: room for all of a warp's
             uint32_t reach = 0;
 #pragma unroll
-            for (int i = 0; i < 16; ++i) reach |= v[i] >= bar_x ? 1u << i : 0u;
-            while (reach) {
-                const int i = __ffs(reach) - 1;
-                reach &= reach - 1;
-                fullest = max(fullest, put_key(list, key_of(i), bar));
+            for (int i = 0; i < 16; ++i) reach |= v[i] >= bar_x && v[i] > -INFINITY ? 1u << i : 0u;
+            int before = __popc(reach);
+#pragma unroll
+            for (int o = 1; o < 32; o *= 2) {
+                const int n = __shfl_up_sync(0xffffffffu, before, o);
+                if ((threadIdx.x & 31) >= o) before += n;
+            }
+            int at = 0;
+            if ((threadIdx.x & 31) == 31) at = atomicAdd(&list.count, before);
+            at = __shfl_sync(0xffffffffu, at, 31) + before - __popc(reach);
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+                if (reach >> i & 1) {
+                    if (at < LIST) list.key[at] = rank_key(v[i], col0 + i / 4 * (4 * TPB) + i % 4);
+                    ++at;
+                }
+        }
+        if (v0 + TPB * 4 < check && v0 + TPB * 4 < vecs) continue;
+        __syncthreads();
+        if (list.count > LIST) {
+            // not all had room: the tiles since the last look once more, the slow way
+            __syncthreads();
+            if (threadIdx.x == 0) list.count = held;
+            __syncthreads();
+#pragma unroll 1
+            for (int u0 = since; u0 <= v0; u0 += TPB * 4) {
+                float u[16];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const float4 f = u0 + j * TPB + (int)threadIdx.x < vecs ? p[u0 + j * TPB] : none;
+                    u[4 * j] = f.x; u[4 * j + 1] = f.y; u[4 * j + 2] = f.z; u[4 * j + 3] = f.w;
+                }
+#pragma unroll 1
+                for (int i = 0; i < 16; ++i) put_step<TPB>(list, k, key_of(u, u0, i));
             }
         }
-        if (settle<16>(list, k, fullest, v0 == 0, key_of)) read_bar();
+        cut_list<TPB>(list, k);
+        read_bar();
+        held = list.count;
+        __syncthreads();
+        since = v0 + TPB * 4;
+        check = 2 * since;
     }
     st = zn_softmax_block<TPB, true>(st, c, part, [] { __syncthreads(); });
-    if (k > 0) cut_list(list, k);
+    if (k > 0 && vecs <= 0) cut_list<TPB>(list, k);
     int kept = list.count;
     if (pieces > 1) {
         // a piece's record: m, s, w, count, then its keys
@@ -245,21 +268,19 @@ __global__ void __launch_bounds__(TPB, 3) scores_kernel(zn_scores_args a, int pi
         if (k > 0) {
             if (threadIdx.x == 0 && bar != 0) list.bar = bar - 1;
             __syncthreads();
-            for (int i0 = 0; i0 < pieces * k; i0 += TPB * 4) {
-                unsigned long long key[4];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int i = i0 + j * TPB + threadIdx.x;
-                    key[j] = i < pieces * k ? __ldcg(reinterpret_cast<const unsigned long long *>(scratch + (r * pieces + i / k) * record + 4) + i % k) : 0ull;
-                }
-                bar = list.bar;
+            const auto key_at = [&](int i) {
+                return i < pieces * k ? __ldcg(reinterpret_cast<const unsigned long long *>(scratch + (r * pieces + i / k) * record + 4) + i % k) : 0ull;
+            };
+            bar = list.bar;
+            for (int i = threadIdx.x; i < pieces * k; i += TPB) put_key(list, key_at(i), bar);
+            __syncthreads();
+            if (list.count > LIST) {
                 __syncthreads();
-                int fullest = 0;
-#pragma unroll
-                for (int j = 0; j < 4; ++j) fullest = max(fullest, put_key(list, key[j], bar));
-                settle<4>(list, k, fullest, false, [&](int i) { return i == 0 ? key[0] : i == 1 ? key[1] : i == 2 ? key[2] : key[3]; });
+                if (threadIdx.x == 0) list.count = 0;
+                __syncthreads();
+                for (int i = threadIdx.x; i - (int)threadIdx.x < pieces * k; i += TPB) put_step<TPB>(list, k, key_at(i));
             }
-            cut_list(list, k);
+            cut_list<TPB>(list, k);
             kept = list.count;
         }
     }
@@ -290,9 +311,10 @@ __global__ void __launch_bounds__(TPB, 3) scores_kernel(zn_scores_args a, int pi
 
 // Gradient: every value by itself, one read and one write of the block.  A block takes 4096 columns of a row, stores 16
 // bytes at a time and loads as wide where both rows stand alike.
-__global__ void __launch_bounds__(TPB) scores_grad_kernel(zn_scores_grad_args a, int pieces, int *status) {
+constexpr int GRAD_TILE = GRAD_TPB * 16;
+__global__ void __launch_bounds__(GRAD_TPB) scores_grad_kernel(zn_scores_grad_args a, int pieces, int *status) {
     const int64_t r = blockIdx.x / pieces;
-    const int64_t lo = (blockIdx.x % pieces) * (int64_t)TILE, hi = min(a.vocab, lo + TILE);
+    const int64_t lo = (blockIdx.x % pieces) * (int64_t)GRAD_TILE, hi = min(a.vocab, lo + GRAD_TILE);
     const float *x = a.logits + r * a.ld;
     float *g = a.grad + r * a.ld_grad;
     int64_t t = a.grad_logprob ? a.tokens[r] : -1;
@@ -319,7 +341,7 @@ __global__ void __launch_bounds__(TPB) scores_grad_kernel(zn_scores_grad_args a,
     float4 v[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-        const int64_t i = j * TPB + threadIdx.x;
+        const int64_t i = j * GRAD_TPB + threadIdx.x;
         if (i >= vecs || none) continue;
         const float *p = x + from + 4 * i;
         if (alike) v[j] = __ldcs(reinterpret_cast<const float4 *>(p));
@@ -331,7 +353,7 @@ __global__ void __launch_bounds__(TPB) scores_grad_kernel(zn_scores_grad_args a,
     if (has_end) ends = x[end];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-        const int64_t i = j * TPB + threadIdx.x, col = from + 4 * i;
+        const int64_t i = j * GRAD_TPB + threadIdx.x, col = from + 4 * i;
         if (i >= vecs) continue;
         float4 o;
         o.x = value(v[j].x, col);
@@ -345,11 +367,12 @@ __global__ void __launch_bounds__(TPB) scores_grad_kernel(zn_scores_grad_args a,
 
 }   // namespace
 
-// Rows alone fill the GPU from two blocks per SM on; fewer are cut into pieces of whole tiles.
+// Threads per row by the vocabulary: a short row is over before many threads have met, so more rows at once do better.
+// Rows alone fill the GPU from two blocks of 256 threads per SM on; fewer are cut into pieces of whole tiles.
 zn_token_plan zn_plan_token_logprobs(size_t rows, size_t vocab, size_t top_k, int sms) {
     zn_token_plan p;
-    p.threads = TPB;
-    const int64_t tiles = (int64_t)((vocab + TILE - 1) / TILE);
+    p.threads = vocab <= 2048 ? 64 : vocab <= 8192 ? 128 : 256;
+    const int64_t tile = p.threads * 16, tiles = ((int64_t)vocab + tile - 1) / tile;
     int64_t pieces = rows > 0 && (int64_t)rows < 2 * sms ? (2 * sms + (int64_t)rows - 1) / (int64_t)rows : 1;
     if (pieces > tiles) pieces = tiles;
     if (pieces > MAX_PIECES) pieces = MAX_PIECES;
@@ -363,15 +386,16 @@ zn_token_plan zn_plan_token_logprobs(size_t rows, size_t vocab, size_t top_k, in
 
 zn_status zn_k_token_logprobs(zn_ctx *ctx, const zn_scores_args &a) {
     const zn_token_plan p = zn_plan_token_logprobs((size_t)a.rows, (size_t)a.vocab, (size_t)a.top_k, ctx->sm_count);
-    const int64_t tiles = (a.vocab + TILE - 1) / TILE;
+    const int64_t tile = p.threads * 16, tiles = (a.vocab + tile - 1) / tile;
     unsigned int *arrivals = nullptr;
-    if (p.share > 1) {                 // at most 2 x SMs rows then: fewer than the lane's counters
+    if (p.share > 1) {                 // fewer than 2 x SMs rows then: fewer than the lane's counters
         ZN_TRY(zn_scratch_reserve(ctx, p.scratch_floats));
         ZN_TRY(zn_lane_counters(ctx, &arrivals));
     }
     zn_launch_scope scope(ctx, ZN_PROF_LOSS, 5.0 * a.rows * a.vocab, 4.0 * a.rows * a.vocab);
-    scores_kernel<<<(unsigned)p.blocks, p.threads, 0, ctx->stream>>>(a, p.share, (tiles + p.share - 1) / p.share * TILE, ctx->scratch, arrivals,
-                                                                     ctx->status_dev);
+    const auto kernel = p.threads == 64 ? scores_kernel<64> : p.threads == 128 ? scores_kernel<128> : scores_kernel<256>;
+    kernel<<<(unsigned)p.blocks, p.threads, 0, ctx->stream>>>(a, p.share, (tiles + p.share - 1) / p.share * tile, ctx->scratch, arrivals,
+                                                              ctx->status_dev);
     ZN_CUDA(ctx, cudaGetLastError());
     return ZN_OK;
 }
@@ -379,14 +403,15 @@ zn_status zn_k_token_logprobs(zn_ctx *ctx, const zn_scores_args &a) {
 zn_token_plan zn_plan_token_logprobs_backward(size_t rows, size_t vocab, int sms) {
     zn_token_plan p;
     (void)sms;
-    p.threads = TPB;
-    p.share = (int)((vocab + TILE - 1) / TILE);
+    p.threads = GRAD_TPB;
+    p.share = (int)((vocab + GRAD_TILE - 1) / GRAD_TILE);
     p.blocks = (int64_t)rows * p.share;
     return p;
 }
 
 zn_status zn_k_token_logprobs_backward(zn_ctx *ctx, const zn_scores_grad_args &a) {
     const zn_token_plan p = zn_plan_token_logprobs_backward((size_t)a.rows, (size_t)a.vocab, ctx->sm_count);
+    if (p.blocks > 0x7fffffff) return zn_fail(ctx, ZN_ERR_SHAPE, "token_logprobs_backward: too many values for one launch");
     zn_launch_scope scope(ctx, ZN_PROF_LOSS, 7.0 * a.rows * a.vocab, 8.0 * a.rows * a.vocab);
     scores_grad_kernel<<<(unsigned)p.blocks, p.threads, 0, ctx->stream>>>(a, p.share, ctx->status_dev);
     ZN_CUDA(ctx, cudaGetLastError());
