@@ -99,7 +99,7 @@ constexpr int BATCH = 8;             // values of a lane on their way at once
 
 struct SortArgs {
     const int32_t *tokens;
-    int32_t *buffer;              // four times `rows`: keys and positions, twice
+    int2 *buffer;                 // twice `rows` pairs of key and position
     float *table;                 // its first `clear` values are set to zero by the blocks that do not sort
     int64_t rows, vocab, clear;
     int passes, bits;
@@ -144,8 +144,7 @@ __global__ void __launch_bounds__(COUNT_THREADS) count_kernel(SortArgs a, int *s
         }
         before = __reduce_add_sync(0xffffffffu, before);
         if (lane == 0) {
-            __stcg(a.buffer + before, (int32_t)mine);
-            __stcg(a.buffer + a.rows + before, r);
+            __stcg(a.buffer + before, make_int2((int)mine, r));
         }
     }
 }
@@ -170,15 +169,16 @@ __global__ void __launch_bounds__(SORT_THREADS) sort_kernel(SortArgs a, int *sta
     zn_cluster_arrive();                                     // all blocks have started
     zn_cluster_wait();
     for (int pass = 0; pass < a.passes; ++pass) {
-        int32_t *src = a.buffer + (pass & 1 ? 0 : 2) * a.rows, *dst = a.buffer + (pass & 1 ? 2 : 0) * a.rows;
+        int2 *src = a.buffer + (pass & 1 ? 0 : a.rows), *dst = a.buffer + (pass & 1 ? a.rows : 0);
         const auto load = [&](int64_t i, uint32_t &key, int32_t &at) {
             if (pass == 0) {
                 const int32_t t = __ldg(a.tokens + i);
                 key = t < 0 || t >= a.vocab ? (uint32_t)a.vocab : (uint32_t)t;
                 at = (int32_t)i;
             } else {
-                key = (uint32_t)__ldcg(src + i);
-                at = __ldcg(src + a.rows + i);
+                const int2 v = __ldcg(src + i);
+                key = (uint32_t)v.x;
+                at = v.y;
             }
         };
         for (int i = threadIdx.x; i < SORT_WARPS * RADIX; i += SORT_THREADS) (&count[0][0])[i] = 0;
@@ -268,8 +268,7 @@ __global__ void __launch_bounds__(SORT_THREADS) sort_kernel(SortArgs a, int *sta
                 if (i0 + 32 * j < hi) {
                     const int digit = digit_of(key[j]);
                     const int64_t to = (int64_t)base[digit] + (held ? count[warp][digit] : 0) + place[j];
-                    __stcg(dst + to, (int32_t)key[j]);
-                    __stcg(dst + a.rows + to, at[j]);
+                    __stcg(dst + to, make_int2((int)key[j], at[j]));
                 }
         }
         zn_cluster_arrive();             // the next pass reads what all blocks wrote
@@ -281,7 +280,7 @@ __global__ void __launch_bounds__(SORT_THREADS) sort_kernel(SortArgs a, int *sta
 
 struct SumArgs {
     const float *grad;
-    const int32_t *key, *at;      // sorted tokens and their positions
+    const int2 *sorted;           // tokens in their order, each with its position
     float *table;
     float *head, *tail;           // per piece: the sum of a run that began before it, of one that goes on behind it
     int64_t rows, vocab, units;
@@ -293,12 +292,12 @@ struct SumArgs {
 };
 
 // The first place of the sorted order whose token is at least `token`, by one warp: 32 probes at a time.
-__device__ int64_t first_at_least(const int32_t *key, int64_t n, int64_t token) {
+__device__ int64_t first_at_least(const int2 *sorted, int64_t n, int64_t token) {
     int64_t lo = 0, hi = n;                           // the answer lies in [lo, hi]
     const int lane = threadIdx.x & 31;
     while (lo < hi) {
         const int64_t step = (hi - lo + 31) / 32, at = lo + step * lane;
-        const unsigned below = __ballot_sync(0xffffffffu, at < hi && __ldcg(key + at) < token);
+        const unsigned below = __ballot_sync(0xffffffffu, at < hi && __ldcg(&sorted[at].x) < token);
         const int last = 31 - __clz(below);           // probes are in order: the ones below come first
         if (below == 0) return lo;
         const int64_t next = lo + step * (last + 1);
@@ -319,12 +318,12 @@ __device__ void clear_rows(const SumArgs &a, int64_t width, int64_t me, int64_t 
         __syncthreads();
         if (threadIdx.x < CLEAR_ROWS / 32) mark[threadIdx.x] = 0;
         if (threadIdx.x < 64) {
-            const int64_t at = first_at_least(a.key, a.rows, threadIdx.x < 32 ? row : end);
+            const int64_t at = first_at_least(a.sorted, a.rows, threadIdx.x < 32 ? row : end);
             if ((threadIdx.x & 31) == 0) range[threadIdx.x >> 5] = at;
         }
         __syncthreads();
         for (int64_t i = range[0] + threadIdx.x; i < range[1]; i += TPB) {
-            const int t = (int)(__ldcg(a.key + i) - row);
+            const int t = (int)(__ldcg(&a.sorted[i].x) - row);
             atomicOr(&mark[t >> 5], 1u << (t & 31));
         }
         __syncthreads();
@@ -351,16 +350,19 @@ __device__ __forceinline__ void sum_piece(const SumArgs &a, int wide, int cuts) 
     const int64_t lo = piece * a.piece, hi = min(a.rows, lo + a.piece);
     const T *g = reinterpret_cast<const T *>(a.grad);
     T *table = reinterpret_cast<T *>(a.table);
-    const int32_t ahead = lo > 0 ? __ldcg(a.key + lo - 1) : -1, behind = hi < a.rows ? __ldcg(a.key + hi) : -1;
+    const int32_t ahead = lo > 0 ? __ldcg(&a.sorted[lo - 1].x) : -1, behind = hi < a.rows ? __ldcg(&a.sorted[hi].x) : -1;
     bool continued = false, begun = false;
     T sum = U::zero();
     for (int64_t i0 = lo; i0 < hi; i0 += 8) {
         int32_t key[9], at[8];
         T v[8], old[8];
 #pragma unroll
-        for (int j = 0; j < 9; ++j) key[j] = i0 + j < hi ? __ldcg(a.key + i0 + j) : -1;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) at[j] = i0 + j < hi ? __ldcg(a.at + i0 + j) : 0;
+        for (int j = 0; j < 8; ++j) {
+            const int2 s = i0 + j < hi ? __ldcg(a.sorted + i0 + j) : make_int2(-1, 0);
+            key[j] = s.x;
+            at[j] = s.y;
+        }
+        key[8] = i0 + 8 < hi ? __ldcg(&a.sorted[i0 + 8].x) : -1;
         // -1 and the count of tokens stand for none: nothing is read or written there
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
@@ -430,7 +432,7 @@ __global__ void __launch_bounds__(TPB) run_join_kernel(SumArgs a, int wide, int 
         return sum;
     };
     const auto put = [&](int64_t piece, T tail, T old, T sum) {
-        const int64_t token = __ldcg(a.key + (piece + 1) * a.piece - 1);
+        const int64_t token = __ldcg(&a.sorted[(piece + 1) * a.piece - 1].x);
         if (lane < wide && live) reinterpret_cast<T *>(a.table)[token * a.units + c] = U::add(old, U::mul(a.scale, U::add(tail, sum)));
     };
     const auto old_of = [&](int64_t token) { return live && a.accumulate ? reinterpret_cast<const T *>(a.table)[token * a.units + c] : U::zero(); };
@@ -438,12 +440,12 @@ __global__ void __launch_bounds__(TPB) run_join_kernel(SumArgs a, int wide, int 
     if (lane == 0) later[warp] = 0;
     const int64_t piece = piece0 + warp, lo = piece * a.piece, hi = lo + a.piece;
     if (hi < a.rows) {
-        const int32_t token = __ldcg(a.key + hi - 1), behind = __ldcg(a.key + hi), ahead = lo > 0 ? __ldcg(a.key + lo - 1) : -1;
+        const int32_t token = __ldcg(&a.sorted[hi - 1].x), behind = __ldcg(&a.sorted[hi].x), ahead = lo > 0 ? __ldcg(&a.sorted[lo - 1].x) : -1;
         if (token < a.vocab && behind == token && ahead != token) {
             int64_t heads = 0;                                               // pieces that begin with the token
             for (;;) {
                 const int64_t p = piece + 1 + heads + lane;
-                const int more = __popc(__ballot_sync(0xffffffffu, p < a.pieces && __ldcg(a.key + p * a.piece) == token));
+                const int more = __popc(__ballot_sync(0xffffffffu, p < a.pieces && __ldcg(&a.sorted[p * a.piece].x) == token));
                 heads += more;
                 if (more < 32) break;
             }
@@ -460,7 +462,7 @@ __global__ void __launch_bounds__(TPB) run_join_kernel(SumArgs a, int wide, int 
         if (warp == 0) {
             T all = sums[0][lane];
             for (int i = 1; i < WARPS; ++i) all = U::add(all, sums[i][lane]);
-            put(piece0 + w, tail_of(piece0 + w), old_of(__ldcg(a.key + (piece0 + w + 1) * a.piece - 1)), all);
+            put(piece0 + w, tail_of(piece0 + w), old_of(__ldcg(&a.sorted[(piece0 + w + 1) * a.piece - 1].x)), all);
         }
         __syncthreads();
     }
@@ -540,7 +542,7 @@ zn_status zn_k_embedding_backward(zn_ctx *ctx, const float *grad_out, const int3
     const zn_token_plan p = zn_plan_embedding_backward(rows, vocab, dim, ctx->sm_count);
     ZN_TRY(zn_scratch_reserve(ctx, p.scratch_floats));
     const bool count = rows <= COUNT_MOST;
-    SortArgs s{tokens, reinterpret_cast<int32_t *>(ctx->scratch), grad_table, (int64_t)rows, (int64_t)vocab, 0, 0, 0, 0};
+    SortArgs s{tokens, reinterpret_cast<int2 *>(ctx->scratch), grad_table, (int64_t)rows, (int64_t)vocab, 0, 0, 0, 0};
     int key_bits = 1;
     while (((int64_t)vocab >> key_bits) != 0) ++key_bits;
     s.passes = count ? 1 : (key_bits + 7) / 8;
@@ -556,8 +558,7 @@ zn_status zn_k_embedding_backward(zn_ctx *ctx, const float *grad_out, const int3
     a.piece = (int)piece_of((int64_t)rows, (int64_t)(dim % 4 == 0 ? dim / 4 : dim), ctx->sm_count);
     a.pieces = ((int64_t)rows + a.piece - 1) / a.piece;
     const int64_t row_pad = ((int64_t)rows + 3) / 4 * 4, dim_pad = ((int64_t)dim + 3) / 4 * 4;
-    int32_t *sorted = s.buffer + (!count && (s.passes - 1) & 1 ? 2 : 0) * (int64_t)rows;
-    a.grad = grad_out; a.key = sorted; a.at = sorted + rows; a.table = grad_table;
+    a.grad = grad_out; a.sorted = s.buffer + (!count && (s.passes - 1) & 1 ? (int64_t)rows : 0); a.table = grad_table;
     a.head = ctx->scratch + 4 * row_pad; a.tail = a.head + a.pieces * dim_pad;
     a.rows = (int64_t)rows; a.vocab = (int64_t)vocab; a.scale = scale; a.accumulate = accumulate ? 1 : 0;
     const int wide = width_of(a.units, TPB), join_wide = width_of(a.units, 32);
