@@ -15,7 +15,8 @@ constexpr int MAX_SHARE = 8, MAX_RING = 3, MAX_WARPS = 16;
 constexpr int HELD = 36;                         // values of a slice that a thread holds in registers
 
 struct Shared {
-    float warp[2][MAX_SHARE * MAX_WARPS][2];     // maximum and sum of every warp of the row's blocks; rows take turns
+    float part[MAX_WARPS][2];                    // maximum and sum of every warp
+    float slice[2][MAX_SHARE][2];                // and of every block of the row; rows take turns
     float ends[MAX_RING][8];                     // the values before and behind the aligned part of the slice
     float weight[MAX_RING], loss_q[MAX_RING];    // sum q log q of the row in this place of the ring
     int state[MAX_RING];                         // what the teacher's entries leave of it
@@ -26,24 +27,50 @@ struct Shared {
 enum { FILL_GRADIENT = 0, FILL_ZERO = 1, FILL_NAN = 2, FILL_EMPTY = 3 };
 enum { ROW_FINE = 0, ROW_NONE = 1, ROW_WRONG = 2, ROW_NAN = 3 };     // nothing to learn; id past the vocabulary; NaN among the logits
 
-// The teacher's entries of a row, by one warp: q = softmax(u / T) over them, the student's logits at their tokens.
-__device__ void read_teacher(const zn_distill_args &a, int64_t r, int lane, float *q, float *xt, int32_t *id, float *together, float *loss_q,
-                             int *state, bool report, int *status) {
-    const float *x = a.logits + r * a.ld;
+// A lane's share of 128 of the teacher's entries.  Their reads depend on one another (an entry, then the student's logit
+// there) and are slow while the rows stream by, so they are started a row ahead.
+struct Entries {
+    int32_t id[4];
+    float u[4], x[4];
+};
+__device__ __forceinline__ void load_ids(Entries &e, const zn_distill_args &a, int64_t r, int j0, int lane) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int j = j0 + lane + 32 * i;
+        e.id[i] = j < a.k ? __ldg(a.ids + r * a.k + j) : -1;
+        e.u[i] = j < a.k ? __ldg(a.teacher + r * a.k + j) : -INFINITY;
+    }
+}
+__device__ __forceinline__ void load_logits(Entries &e, const zn_distill_args &a, int64_t r) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) e.x[i] = e.id[i] >= 0 && e.id[i] < a.vocab && e.u[i] != -INFINITY ? a.logits[r * a.ld + e.id[i]] : 0.f;
+}
+
+// The teacher's entries of a row, by one warp: q = softmax(u / T) over them, the student's logits at their tokens.  The
+// first 128 have been loaded.
+__device__ void read_teacher(const zn_distill_args &a, int64_t r, Entries e, int lane, float *q, float *xt, int32_t *id, float *together,
+                             float *loss_q, int *state, bool report, int *status) {
     const float inv_t = 1.f / a.temperature;
     float um = -INFINITY;
     bool wrong = false, nan = false;
-    for (int j = lane; j < a.k; j += 32) {
-        const int32_t t = a.ids[r * a.k + j];
-        const float u = a.teacher[r * a.k + j];
-        const bool entry = t >= 0 && u != -INFINITY;
-        wrong = wrong || (entry && t >= a.vocab);
-        nan = nan || (entry && !(u < INFINITY));
-        const bool fine = entry && t < a.vocab;
-        id[j] = fine ? t : -1;
-        xt[j] = fine ? x[t] : 0.f;
-        q[j] = u;
-        if (entry) um = fmaxf(um, u);
+    for (int j0 = 0; j0 < a.k; j0 += 128) {
+        if (j0 > 0) {
+            load_ids(e, a, r, j0, lane);
+            load_logits(e, a, r);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int j = j0 + lane + 32 * i;
+            const bool entry = e.id[i] >= 0 && e.u[i] != -INFINITY, fine = entry && e.id[i] < a.vocab;
+            wrong = wrong || (entry && !fine);
+            nan = nan || (entry && !(e.u[i] < INFINITY));
+            if (entry) um = fmaxf(um, e.u[i]);
+            if (j < a.k) {
+                id[j] = fine ? e.id[i] : -1;
+                xt[j] = e.x[i];
+                q[j] = e.u[i];
+            }
+        }
     }
     um = zn_warp_max(um);
     wrong = __any_sync(0xffffffffu, wrong);
@@ -148,15 +175,25 @@ __global__ void __launch_bounds__(THREADS + 64 + 32 * MAX_RING) distill_kernel(z
     if (threadIdx.x >= THREADS) {
         const int helper = (threadIdx.x - THREADS) >> 5;
         int place = 0, turn = 0;
+        Entries entries;
+        if (helper < ring && cluster + helper * clusters < a.rows) {
+            load_ids(entries, a, cluster + helper * clusters, 0, lane);
+            load_logits(entries, a, cluster + helper * clusters);
+        }
         for (int64_t r = cluster; r < a.rows; r += clusters) {
             float *q = teacher + place * 4 * a.k, *xt = q + a.k, *together = q + 3 * a.k;
             int32_t *id = reinterpret_cast<int32_t *>(q + 2 * a.k);
-            if (turn > 0 && (helper == place || helper == MAX_RING)) zn_bar_wait(&s.free_[place], (turn - 1) & 1, status, 21);
             if (helper == place) {
-                read_teacher(a, r, lane, q, xt, id, together, &s.loss_q[place], &s.state[place], rank == 0, status);
+                const int64_t after = r + ring * clusters;
+                const Entries now = entries;
+                if (after < a.rows) load_ids(entries, a, after, 0, lane);
+                if (turn > 0) zn_bar_wait(&s.free_[place], (turn - 1) & 1, status, 21);
+                read_teacher(a, r, now, lane, q, xt, id, together, &s.loss_q[place], &s.state[place], rank == 0, status);
                 __syncwarp();
                 if (lane == 0) zn_bar_arrive(&s.full[place]);
+                if (after < a.rows) load_logits(entries, a, after);
             } else if (helper == MAX_RING) {
+                if (turn > 0) zn_bar_wait(&s.free_[place], (turn - 1) & 1, status, 21);
                 lay_out(r, x, from, vecs, mine, place);
                 const float w = a.weights ? a.weights[r] : 1.f;
                 if (lane == 0) {
@@ -243,6 +280,7 @@ __global__ void __launch_bounds__(THREADS + 64 + 32 * MAX_RING) distill_kernel(z
                 float part[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int j = 0; j < HELD; ++j) {
+                    if (j / 4 * THREADS >= vecs) break;                // no thread has more
                     v[j] = zn_exp2(__fmul_rn(v[j] - base, c));
                     part[j & 3] += v[j];
                 }
@@ -271,28 +309,32 @@ __global__ void __launch_bounds__(THREADS + 64 + 32 * MAX_RING) distill_kernel(z
                         zn_softmax_add<1, false>(st, o, o[0], c);
                     }
             }
-            // over the warp, then over all warps of the row's blocks: each sends what it has to every block
+            // over the warp, over the block by its first warp, which sends what they come to to every block of the row
             const float own_m = st.m;
             zn_softmax_raise<false>(st, zn_warp_max(st.m), c);
             st.s = zn_warp_sum(st.s);
-            if (threadIdx.x == 0) zn_bar_expect(&s.met[side], 8u * WARPS * (uint32_t)share);
-            if (lane < share) zn_cluster_send(s.warp[side][rank * WARPS + (threadIdx.x >> 5)], st.m, st.s, &s.met[side], lane);
+            if (lane == 0) {
+                s.part[threadIdx.x >> 5][0] = st.m;
+                s.part[threadIdx.x >> 5][1] = st.s;
+            }
+            zn_part_sync(THREADS);
+            if (threadIdx.x < 32) {
+                zn_softmax all{-INFINITY, 0.f, 0.f};
+                if (lane < WARPS) all = {s.part[lane][0], s.part[lane][1], 0.f};
+                zn_softmax_raise<false>(all, zn_warp_max(all.m), c);
+                all.s = zn_warp_sum(all.s);
+                if (lane == 0) zn_bar_expect(&s.met[side], 8u * (uint32_t)share);
+                if (lane < share) zn_cluster_send(s.slice[side][rank], all.m, all.s, &s.met[side], lane);
+            }
             zn_bar_wait(&s.met[side], side_phase, status, 23);       // from here on nobody still needs the logits in global memory
-            const int all = share * WARPS;
-            float am[MAX_SHARE * WARPS / 32 + 1], m = -INFINITY, sum = 0.f;
+            zn_softmax row{-INFINITY, 0.f, 0.f};
+            if (lane < share) row = {s.slice[side][lane][0], s.slice[side][lane][1], 0.f};
+            const float m = zn_warp_max(row.m);
+            zn_softmax_raise<false>(row, m, c);
+            float sum = row.s;
 #pragma unroll
-            for (int j = 0; j < MAX_SHARE * WARPS / 32 + 1; ++j) {
-                const int i = lane + 32 * j;
-                am[j] = i < all ? s.warp[side][i][0] : -INFINITY;
-                m = fmaxf(m, am[j]);
-            }
-            m = zn_warp_max(m);
-#pragma unroll
-            for (int j = 0; j < MAX_SHARE * WARPS / 32 + 1; ++j) {
-                const int i = lane + 32 * j;
-                if (i < all) sum += s.warp[side][i][1] * zn_exp2(am[j] == m ? 0.f : __fmul_rn(am[j] - m, c));
-            }
-            sum = zn_warp_sum(sum);
+            for (int o = MAX_SHARE / 2; o > 0; o /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+            sum = __shfl_sync(0xffffffffu, sum, 0);
             side_phase ^= side;
             side ^= 1;
             const int verdict = w == 0.f || state == ROW_NONE || state == ROW_WRONG ? FILL_ZERO
