@@ -178,7 +178,7 @@ ZN_API zn_status zn_evaluate_classification(zn_ctx *ctx, const float *outputs, c
  * and writes nothing out of range, its row gets what the entry point says below, and the next call that waits for the
  * device (zn_end_command_batch, zn_tensor_download, any call with a host operand) returns ZN_ERR_INVALID_VALUE.
  *
- * Blocks of logits have a row pitch `ld` >= vocab in floats; columns from vocab to ld are neither read nor written.
+ * Blocks of logits have a row pitch `ld` >= vocab in floats (2^30 at most); columns from vocab to ld are neither read nor written.
  * Outputs may not overlap inputs or each other unless an entry point says so (ZN_ERR_INVALID_VALUE).  rows == 0 does
  * nothing, except that zn_embedding_backward still clears the table it was to write.  All sums, maxima and softmax statistics are formed in f32 whatever the context's precision mode, each in a
  * fixed order: the same call gives the same bits. */

@@ -22,6 +22,7 @@ def plan(op, a, b, c, sms=148):
     (0, 4, 0, 8, SHAPE), (0, 4, 8, 0, SHAPE), (0, BIG, 8, 8, SHAPE), (0, 4, BIG - 1, BIG - 1, SHAPE),
     (1, 4, 0, 8, SHAPE), (1, 4, 8, 0, SHAPE), (1, BIG - 1, 8, BIG - 1, SHAPE),
     (2, 4, 0, 0, SHAPE), (2, 4, 100, 129, INVALID), (2, BIG, 100, 0, SHAPE),
+    (2, 1, (1 << 30) + 1, 0, SHAPE), (3, 1, (1 << 30) + 1, 0, SHAPE), (4, 1, (1 << 30) + 1, 1, SHAPE),
     (3, 4, 0, 0, SHAPE), (4, 4, 0, 1, SHAPE), (4, 4, 100, 0, SHAPE), (4, 4, 100, 513, SHAPE),
     (5, 0, 8, 32, SHAPE), (5, 8, 0, 32, SHAPE), (5, 8, 8, 48, INVALID), (5, 8, 8, 0, INVALID),
     (6, 1, 0, 8, SHAPE), (6, 1, 8, 0, SHAPE), (6, 1, BIG, 8, SHAPE), (7, 1, 1, 1, INVALID), (-1, 1, 1, 1, INVALID),

@@ -188,7 +188,7 @@ def check_scores(got, want, k):
 
 SCORES = [(1, 1, 1, 1.0, 1), (1, 5, 5, 2.0, 8), (3, 17, 20, 0.7, 17), (2, 129, 129, 1.0, 128), (5, 1000, 1003, 1.3, 3), (300, 999, 999, 1.0, 10),
           (1, 131072, 131072, 0.8, 20), (7, 50001, 50001, 1.0, 128), (2, 200003, 200010, 3.0, 64), (700, 4099, 4100, 1.0, 5),
-          (1500, 257, 260, 0.5, 40), (900, 3000, 3001, 1.0, 100), (600, 1025, 1027, 1.0, 64), (600, 2048, 2048, 0.9, 128), (3, 8000, 8000, 1.0, 65), (64, 32768, 32768, 1.0, 0), (640, 20001, 20001, 1.0, 31), (13, 8191, 8192, 1.0, 1)]
+          (1500, 257, 260, 0.5, 40), (900, 3000, 3001, 1.0, 100), (600, 1025, 1027, 1.0, 64), (600, 2048, 2048, 0.9, 128), (3, 8000, 8000, 1.0, 65), (70000, 3, 3, 1.0, 2), (64, 32768, 32768, 1.0, 0), (640, 20001, 20001, 1.0, 31), (13, 8191, 8192, 1.0, 1)]
 
 
 @pytest.mark.parametrize("rows,vocab,ld,t,k", SCORES)
@@ -300,7 +300,7 @@ def test_scores_misaligned(be):
 
 
 GRADS = [(1, 1, 1, 1, 1.0), (1, 5, 5, 7, 2.0), (3, 17, 20, 20, 0.7), (5, 1000, 1003, 1000, 1.3), (300, 999, 999, 999, 1.0),
-         (1, 131072, 131072, 131072, 0.8), (7, 50001, 50001, 50003, 1.0), (700, 4099, 4100, 4100, 1.0), (1500, 257, 260, 263, 0.5)]
+         (1, 131072, 131072, 131072, 0.8), (7, 50001, 50001, 50003, 1.0), (700, 4099, 4100, 4100, 1.0), (1500, 257, 260, 263, 0.5), (70000, 3, 3, 4, 1.0)]
 
 
 @pytest.mark.parametrize("which", ["both", "logprob", "entropy"])
@@ -395,7 +395,7 @@ def run_distill(be, buf, ids, u, vocab, t, w, ld_grad, in_place=False):
 
 DISTILL = [(1, 1, 1, 1, 1, 1.0), (1, 5, 5, 7, 3, 2.0), (3, 17, 20, 20, 17, 0.7), (5, 1000, 1003, 1001, 512, 1.3), (300, 999, 999, 999, 10, 1.0),
            (1, 131072, 131072, 131072, 64, 2.0), (7, 50001, 50001, 50003, 20, 1.0), (2, 200003, 200010, 200003, 100, 3.0),
-           (700, 4099, 4100, 4101, 5, 1.0), (1500, 257, 260, 260, 40, 0.5), (40, 32768, 32768, 32768, 16, 4.0), (2, 460001, 460001, 460001, 9, 1.0)]
+           (700, 4099, 4100, 4101, 5, 1.0), (1500, 257, 260, 260, 40, 0.5), (40, 32768, 32768, 32768, 16, 4.0), (2, 460001, 460001, 460001, 9, 1.0), (70000, 3, 3, 3, 2, 1.0), (600, 20000, 20000, 20000, 300, 1.0), (200, 150001, 150001, 150001, 7, 1.0)]
 
 
 @pytest.mark.parametrize("rows,vocab,ld,ld_grad,k,t", DISTILL)
@@ -469,6 +469,40 @@ def test_distill_of_odd_rows(be, vocab):
     assert np.allclose(g[2], want, rtol=64 * ref.U, atol=0)
     (_, _), (grad, err) = ref.distill_loss(x[[3, 8]], ids[[3, 8]], u[[3, 8]], 2.0, w[[3, 8]])
     ref.check(g[[3, 8]], grad, err)
+
+
+@pytest.mark.parametrize("vocab", [130, 9003, 40001, 160003])
+def test_distill_rows_of_all_kinds_in_one_call(be, vocab):
+    """What a row is does not show in the next one of the same block: many rows, every fifth with something odd."""
+    rng = np.random.default_rng(27)
+    rows, k = 400, 5
+    x = padded(rng, rows, vocab, vocab)
+    ids, u = teacher(rng, rows, vocab, k)
+    ids[:, 0] = 7
+    w = np.ones(rows, F32)
+    kind = np.where(np.arange(rows) % 5 == 2, rng.integers(1, 6, rows), 0)
+    for r in np.nonzero(kind)[0]:
+        if kind[r] == 1:
+            x[r, vocab // 2] = np.nan
+        elif kind[r] == 2:
+            w[r] = 0
+            x[r, 1] = np.inf
+        elif kind[r] == 3:
+            ids[r] = -1
+        elif kind[r] == 4:
+            x[r] = NINF
+        else:
+            u[r, 0] = np.nan
+    loss, g = run_distill(be, x, ids, u, vocab, 1.0, w, vocab)
+    again, g2 = run_distill(be, x, ids, u, vocab, 1.0, w, vocab, in_place=True)
+    assert np.array_equal(loss, again, equal_nan=True) and np.array_equal(g, g2, equal_nan=True)
+    fine = kind == 0
+    (l, le), (grad, ge) = ref.distill_loss(x[fine], ids[fine], u[fine], 1.0, w[fine])
+    ref.check(loss[fine], l, le)
+    ref.check(g[fine], grad, ge)
+    assert np.isnan(loss[(kind == 1) | (kind == 5)]).all() and np.isnan(g[(kind == 1) | (kind == 5)]).all()
+    assert not loss[(kind == 2) | (kind == 3)].any() and not g[(kind == 2) | (kind == 3)].any()
+    assert np.all(loss[kind == 4] == np.inf) and np.isfinite(g[kind == 4]).all()
 
 
 def test_distill_against_differences(be):
@@ -758,6 +792,52 @@ def test_two_contexts_at_once():
             assert np.array_equal(s[i].numpy(), v)
     a.deinit()
     b.deinit()
+
+
+def test_calls_between_submitted_training_steps(be):
+    """Steps in flight use the context's other streams and their scratch; calls in between give what they give alone, and
+    the network trains as it does undisturbed."""
+    rng = np.random.default_rng(28)
+    rows, vocab, k = 3, 60001, 20
+    x, tok = padded(rng, rows, vocab, vocab), rng.integers(0, vocab, rows).astype(I32)
+    emb, g = zipf_tokens(rng, 5000, 300), rng.standard_normal((5000, 64)).astype(F32)
+    dx, dk, de, dg = be.tensor(x), be.tensor(tok, I32), be.tensor(emb, I32), be.tensor(g)
+    lp, tt, tl, dt = be.tensor(rows), be.tensor(rows * k, I32), be.tensor(rows * k), be.tensor(300 * 64)
+    xin, t = rng.standard_normal((256, 96)).astype(F32), rng.standard_normal((256, 40)).astype(F32)
+    w = [rng.standard_normal((96, 80)).astype(F32) * F32(0.1), rng.standard_normal((80, 40)).astype(F32) * F32(0.1)]
+
+    def train(between):
+        net = zn.Network(be, zn.Precision.FP32_SIMT)
+        net.addDense(96, 80, "relu")
+        net.addDense(80, 40, "linear")
+        for i in range(2):
+            net.setWeights(i, w[i], np.zeros(w[i].shape[1], F32))
+        net.setOptimizer(zn.Adam())
+        losses, flying = [], 0
+        for _ in range(8):
+            net.submitStep(hx, ht, 256, 1e-3, zn.Loss.mse)
+            flying += 1
+            if between:
+                be.tokenLogProbs(dx, dk, rows, vocab, logprob=lp, top_k=k, top_tokens=tt, top_logprobs=tl)
+                be.embeddingBackward(dg, de, dt, 5000, 300, 64)
+            if flying == 2:
+                losses.append(net.waitStep())
+                flying -= 1
+        losses.append(net.waitStep())
+        out = [net.getWeights(i)[0] for i in range(2)]
+        net.deinit()
+        return losses, out
+
+    hx, ht = be.host_alloc(xin.shape), be.host_alloc(t.shape)
+    hx[:], ht[:] = xin, t
+    alone, weights = train(False)
+    mixed, mixed_weights = train(True)
+    assert alone == mixed and all(np.array_equal(a, b) for a, b in zip(weights, mixed_weights))
+    want = ref.token_logprobs(x, tok, 1.0, k)
+    ref.check(lp.numpy(), *want[0])
+    assert np.array_equal(tt.numpy((rows, k)), want[3])
+    ref.check(dt.numpy((300, 64)), *ref.embedding_backward(g, emb, 300, 1.0))
+    free(dx, dk, de, dg, lp, tt, tl, dt)
 
 
 def test_small_call_after_a_large_one_in_the_same_scratch(be):

@@ -340,7 +340,7 @@ __global__ void __launch_bounds__(THREADS + 64 + 32 * MAX_RING) distill_kernel(z
             const int verdict = w == 0.f || state == ROW_NONE || state == ROW_WRONG ? FILL_ZERO
                                 : !(sum >= 0.f) || state == ROW_NAN ? FILL_NAN : m == -INFINITY ? FILL_EMPTY : FILL_GRADIENT;
             float *g = a.grad ? a.grad + r * a.ld_grad + lo : nullptr;
-            const bool copy_out = WHOLE && g && verdict == FILL_GRADIENT && ((reinterpret_cast<uintptr_t>(g + from)) & 15) == 0;
+            const bool copy_out = WHOLE && g && verdict == FILL_GRADIENT && vecs > 0 && ((reinterpret_cast<uintptr_t>(g + from)) & 15) == 0;
             if (threadIdx.x == 0) {
                 s.m[place] = m;
                 s.s[place] = sum;

@@ -479,9 +479,10 @@ constexpr size_t CLEAR_FIRST = (size_t)24 << 20, CLEAR_FIRST_COUNT = (size_t)4 <
 bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 // Rows of the sorted order per piece: so many that about two thousand threads per SM have one, eight at least.
+constexpr int64_t MOST_IN_PIECE = 1 << 20;
 int64_t piece_of(int64_t rows, int64_t units, int sms) {
     const int64_t piece = (rows * units / ((int64_t)sms * 2048) + 7) / 8 * 8;
-    return piece < 8 ? 8 : piece;
+    return piece < 8 ? 8 : piece < MOST_IN_PIECE ? piece : MOST_IN_PIECE;
 }
 
 }   // namespace

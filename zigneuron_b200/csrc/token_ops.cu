@@ -14,6 +14,15 @@ zn_status check_sizes(zn_ctx *ctx, const char *op, size_t a, size_t b, size_t c)
     return ZN_OK;
 }
 
+// Columns of a row of logits are counted in 32 bits, some of them past its end.
+constexpr size_t MAX_PITCH = (size_t)1 << 30;
+zn_status check_logits(zn_ctx *ctx, const char *op, size_t rows, size_t vocab, size_t ld) {
+    if (vocab == 0) return zn_fail(ctx, ZN_ERR_SHAPE, "%s: empty vocabulary", op);
+    if (ld < vocab) return zn_fail(ctx, ZN_ERR_SHAPE, "%s: the row pitch %zu is below the vocabulary %zu", op, ld, vocab);
+    if (ld > MAX_PITCH) return zn_fail(ctx, ZN_ERR_SHAPE, "%s: rows more than 2^30 values apart", op);
+    return check_sizes(ctx, op, rows, ld, 1);
+}
+
 zn_status check_group(zn_ctx *ctx, const char *op, size_t group) {
     if (group != 32 && group != 64 && group != 128)
         return zn_fail(ctx, ZN_ERR_INVALID_VALUE, "%s: groups of %zu weights (32, 64 or 128 are taken)", op, group);
@@ -135,9 +144,7 @@ extern "C" zn_status zn_token_logprobs(zn_ctx *ctx, const float *logits, size_t 
                                        float *row_stats, int32_t *top_tokens, float *top_logprobs) {
     const char *op = "token_logprobs";
     if (!ctx) return ZN_ERR_NOT_INITIALIZED;
-    if (vocab == 0) return zn_fail(ctx, ZN_ERR_SHAPE, "%s: empty vocabulary", op);
-    if (ld < vocab) return zn_fail(ctx, ZN_ERR_SHAPE, "%s: the row pitch %zu is below the vocabulary %zu", op, ld, vocab);
-    ZN_TRY(check_sizes(ctx, op, rows, ld, 1));
+    ZN_TRY(check_logits(ctx, op, rows, vocab, ld));
     ZN_TRY(check_temperature(ctx, op, temperature));
     if (top_k > ZN_TOP_MAX) return zn_fail(ctx, ZN_ERR_INVALID_VALUE, "%s: %zu alternatives, at most %d are taken", op, top_k, (int)ZN_TOP_MAX);
     if (rows == 0) return ZN_OK;
@@ -164,10 +171,8 @@ extern "C" zn_status zn_token_logprobs_backward(zn_ctx *ctx, const float *logits
                                                 size_t vocab, float temperature) {
     const char *op = "token_logprobs_backward";
     if (!ctx) return ZN_ERR_NOT_INITIALIZED;
-    if (vocab == 0) return zn_fail(ctx, ZN_ERR_SHAPE, "%s: empty vocabulary", op);
-    if (ld < vocab || ld_grad < vocab) return zn_fail(ctx, ZN_ERR_SHAPE, "%s: a row pitch is below the vocabulary %zu", op, vocab);
-    ZN_TRY(check_sizes(ctx, op, rows, ld, 1));
-    ZN_TRY(check_sizes(ctx, op, rows, ld_grad, 1));
+    ZN_TRY(check_logits(ctx, op, rows, vocab, ld));
+    ZN_TRY(check_logits(ctx, op, rows, vocab, ld_grad));
     ZN_TRY(check_temperature(ctx, op, temperature));
     if (rows == 0) return ZN_OK;
     if (!logits || !row_stats || !grad_logits) return zn_fail(ctx, ZN_ERR_INVALID_VALUE, "%s: null operand", op);
@@ -195,11 +200,10 @@ extern "C" zn_status zn_distill_loss(zn_ctx *ctx, const float *logits, size_t ld
                                      const float *row_weights, float *row_loss, float *grad_logits, size_t ld_grad) {
     const char *op = "distill_loss";
     if (!ctx) return ZN_ERR_NOT_INITIALIZED;
-    if (vocab == 0) return zn_fail(ctx, ZN_ERR_SHAPE, "%s: empty vocabulary", op);
-    if (ld < vocab || (grad_logits && ld_grad < vocab)) return zn_fail(ctx, ZN_ERR_SHAPE, "%s: a row pitch is below the vocabulary %zu", op, vocab);
+    ZN_TRY(check_logits(ctx, op, rows, vocab, ld));
+    if (grad_logits) ZN_TRY(check_logits(ctx, op, rows, vocab, ld_grad));
     if (k == 0 || k > ZN_TEACHER_MAX) return zn_fail(ctx, ZN_ERR_SHAPE, "%s: teacher lists of %zu entries (1..%d are taken)", op, k, (int)ZN_TEACHER_MAX);
-    ZN_TRY(check_sizes(ctx, op, rows, ld, k));
-    if (grad_logits) ZN_TRY(check_sizes(ctx, op, rows, ld_grad, 1));
+    ZN_TRY(check_sizes(ctx, op, rows, k, 1));
     ZN_TRY(check_temperature(ctx, op, temperature));
     if (rows == 0) return ZN_OK;
     if (!logits || !teacher_tokens || !teacher_logits) return zn_fail(ctx, ZN_ERR_INVALID_VALUE, "%s: null operand", op);
@@ -277,19 +281,18 @@ extern "C" zn_status zn_debug_token_plan(int32_t op, size_t a, size_t b, size_t 
         p = zn_plan_embedding_backward(a, b, c, sms);
         break;
     case 2:
-        if (b == 0) return ZN_ERR_SHAPE;
+        ZN_TRY(check_logits(nullptr, "", a, b, b));
         if (c > ZN_TOP_MAX) return ZN_ERR_INVALID_VALUE;
-        ZN_TRY(check_sizes(nullptr, "", a, b, 1));
         p = zn_plan_token_logprobs(a, b, c, sms);
         break;
     case 3:
-        if (b == 0) return ZN_ERR_SHAPE;
-        ZN_TRY(check_sizes(nullptr, "", a, b, 1));
+        ZN_TRY(check_logits(nullptr, "", a, b, b));
         p = zn_plan_token_logprobs_backward(a, b, sms);
         break;
     case 4:
-        if (b == 0 || c == 0 || c > ZN_TEACHER_MAX) return ZN_ERR_SHAPE;
-        ZN_TRY(check_sizes(nullptr, "", a, b, c));
+        ZN_TRY(check_logits(nullptr, "", a, b, b));
+        if (c == 0 || c > ZN_TEACHER_MAX) return ZN_ERR_SHAPE;
+        ZN_TRY(check_sizes(nullptr, "", a, c, 1));
         p = zn_plan_distill(a, b, c, sms);
         break;
     case 5:
