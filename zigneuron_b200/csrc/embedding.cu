@@ -340,7 +340,7 @@ __device__ void clear_rows(const SumArgs &a, int64_t width, int64_t me, int64_t 
 
 // A group of `wide` threads sums one piece of the sorted order, each thread one unit of the rows, eight rows on their way,
 // and with them what the table holds at the rows that get their sum here.
-template <bool VEC>
+template <bool VEC, bool ADD>
 __device__ __forceinline__ void sum_piece(const SumArgs &a, int wide, int cuts) {
     using U = Unit<VEC>;
     using T = typename U::type;
@@ -368,7 +368,7 @@ __device__ __forceinline__ void sum_piece(const SumArgs &a, int wide, int cuts) 
         for (int j = 0; j < 8; ++j) {
             const bool live = key[j] >= 0 && key[j] < a.vocab;
             v[j] = live ? __ldcs(g + at[j] * a.units + c) : U::zero();
-            old[j] = live && a.accumulate && key[j + 1] != key[j] ? table[key[j] * a.units + c] : U::zero();
+            old[j] = ADD && live && key[j + 1] != key[j] ? table[key[j] * a.units + c] : U::zero();
         }
         if (!begun) {
             continued = key[0] == ahead;
@@ -382,21 +382,21 @@ __device__ __forceinline__ void sum_piece(const SumArgs &a, int wide, int cuts) 
             const bool last = i0 + j + 1 == hi;
             if (continued) reinterpret_cast<T *>(a.head)[piece * a.units + c] = sum;
             else if (last && behind == key[j]) reinterpret_cast<T *>(a.tail)[piece * a.units + c] = sum;
-            else table[key[j] * a.units + c] = U::add(old[j], U::mul(a.scale, sum));
+            else table[key[j] * a.units + c] = ADD ? U::add(old[j], U::mul(a.scale, sum)) : U::mul(a.scale, sum);
             continued = false;
             sum = U::zero();
         }
     }
 }
 
-template <bool VEC>
-__global__ void __launch_bounds__(TPB, VEC ? 2 : 4) run_sum_kernel(SumArgs a, int wide, int cuts) {
+template <bool VEC, bool ADD>
+__global__ void __launch_bounds__(TPB, !VEC ? 4 : ADD ? 2 : 3) run_sum_kernel(SumArgs a, int wide, int cuts) {
     zn_pdl_release();
     zn_pdl_wait();
     // every block clears a share; half of them before their sums and half after, so that both go on at any time
     const bool clears = a.clear_from < a.vocab_rows, early = (blockIdx.x & 1) != 0;
     if (clears && early) clear_rows(a, a.units * (VEC ? 4 : 1), blockIdx.x, gridDim.x);
-    sum_piece<VEC>(a, wide, cuts);
+    sum_piece<VEC, ADD>(a, wide, cuts);
     if (clears && !early) clear_rows(a, a.units * (VEC ? 4 : 1), blockIdx.x, gridDim.x);
 }
 
@@ -599,10 +599,10 @@ zn_status zn_k_embedding_backward(zn_ctx *ctx, const float *grad_out, const int3
     }
     const dim3 sums((unsigned)(sum_blocks > late ? sum_blocks : late)), joins((unsigned)join_blocks), block(TPB);
     if (vec) {
-        ZN_CUDA(ctx, zn_launch_pdl(run_sum_kernel<true>, sums, block, 0, ctx->stream, a, wide, (int)cuts));
+        ZN_CUDA(ctx, zn_launch_pdl(accumulate ? run_sum_kernel<true, true> : run_sum_kernel<true, false>, sums, block, 0, ctx->stream, a, wide, (int)cuts));
         ZN_CUDA(ctx, zn_launch_pdl(run_join_kernel<true>, joins, block, 0, ctx->stream, a, join_wide, (int)join_cuts));
     } else {
-        ZN_CUDA(ctx, zn_launch_pdl(run_sum_kernel<false>, sums, block, 0, ctx->stream, a, wide, (int)cuts));
+        ZN_CUDA(ctx, zn_launch_pdl(accumulate ? run_sum_kernel<false, true> : run_sum_kernel<false, false>, sums, block, 0, ctx->stream, a, wide, (int)cuts));
         ZN_CUDA(ctx, zn_launch_pdl(run_join_kernel<false>, joins, block, 0, ctx->stream, a, join_wide, (int)join_cuts));
     }
     return ZN_OK;
