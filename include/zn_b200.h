@@ -4,7 +4,8 @@
  *
  * The library slots in below ZigNeuron's `Backend` (src/backend.zig): every
  * entry point names the reference function whose CUDA arm it provides.  The
- * interface is plain C: opaque handles, float pointers and sizes.  Slices
+ * interface is plain C: opaque handles, float pointers and sizes (the token-model
+ * operators, which the reference lacks, add int32 ids and packed 4-bit weights).  Slices
  * (`[]f32`) of the reference become `pointer, element count` or explicit
  * dimensions.
  *

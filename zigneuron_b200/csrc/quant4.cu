@@ -5,6 +5,10 @@
 // into bf16 two at a time: a code in the low bits of the bf16 number 128 is 128 + code exactly, and code - 8 after one
 // subtraction.  x keeps all its 24 bits as the sum of three bf16 numbers, which take three columns of the tile; a product
 // of two bf16 numbers is exact in f32, so the only roundings are those of the f32 sums.  A group's sum is scaled once.
+//
+// Measured, 65,536 x 8192 weights in groups of 128 (288 MB, 44 us of HBM): one row 76 us, bound by the codes' conversion (51 %
+// of the integer pipe's cycles; without it 58 us); eight rows 107 us, bound by the matrix steps (three parts of eight rows:
+// 24 columns; without the conversion still 101 us).  4096 x 4096, one row: 10.2 us, latency.
 #include <cuda.h>
 
 #include "zn_token.cuh"
