@@ -17,30 +17,6 @@ __device__ __forceinline__ float zn_warp_max(float v) {       // NaN only where 
 // Records a token id outside the vocabulary in the context's status word; the first code stays.
 __device__ __forceinline__ void zn_bad_token(int *status) { atomicCAS_system(status, 0, (int)ZN_DEVICE_BAD_TOKEN); }
 
-// Sums and maxima of a block of THREADS threads, valid in every thread.  `part` holds one value per warp.
-template <int THREADS>
-__device__ __forceinline__ float zn_block_sum(float v, float *part) {
-    v = zn_warp_sum(v);
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = v;
-    __syncthreads();
-    float s = 0.f;
-#pragma unroll
-    for (int i = 0; i < THREADS / 32; ++i) s += part[i];
-    return s;
-}
-template <int THREADS>
-__device__ __forceinline__ float zn_block_max(float v, float *part) {
-    v = zn_warp_max(v);
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = v;
-    __syncthreads();
-    float s = part[0];
-#pragma unroll
-    for (int i = 1; i < THREADS / 32; ++i) s = fmaxf(s, part[i]);
-    return s;
-}
-
 // 2^v, at most two steps off; results below 2^-126 become zero.
 __device__ __forceinline__ float zn_exp2(float v) {
     float r;
