@@ -128,8 +128,8 @@ for _name, (_res, _args) in SIGNATURES.items():
 
 def ptr(x, dtype=np.float32):
     """void* for a numpy array (host), a DeviceTensor, an int device address, or None."""
-    if x is None:
-        return None
+    if x is None or type(x) is int:
+        return x
     if isinstance(x, np.ndarray):
         if x.dtype != dtype or not x.flags["C_CONTIGUOUS"]:
             raise TypeError(f"operands must be C-contiguous {np.dtype(dtype).name} arrays")

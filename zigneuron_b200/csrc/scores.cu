@@ -14,6 +14,12 @@ __device__ __forceinline__ unsigned long long rank_key(float x, int64_t c) {
     return x == -INFINITY ? 0ull : ((unsigned long long)u << 32) | (uint32_t)(0xffffffffu - (uint32_t)c);
 }
 
+// The logit of a key, which is not "none".
+__device__ __forceinline__ float key_logit(unsigned long long key) {
+    const uint32_t u = (uint32_t)(key >> 32);
+    return __uint_as_float((u & 0x80000000u) ? u & 0x7fffffffu : ~u);
+}
+
 // The k largest keys seen by a block.  Keys above the bar go into a list; when it is half full it is sorted and cut to k,
 // and the bar rises to the k-th.  The result does not depend on the order in which keys arrive: keys are distinct.
 // `count` and `bar` are read by all threads between barriers only.
@@ -110,7 +116,11 @@ __global__ void __launch_bounds__(TPB, 1536 / TPB) scores_kernel(zn_scores_args 
     const float c = 1.4426950408889634f / a.temperature;
     const int k = a.top_k;
     zn_softmax st{-INFINITY, 0.f, 0.f};
+    int64_t token = -1;
+    float given = 0.f;                   // the logit of the row's token, asked for early
     if (threadIdx.x == 0) {
+        if (a.logprob) token = a.tokens[r];
+        if (token >= 0 && token < a.vocab) given = x[token];
         list.count = 0;
         list.bar = 0;
     }
@@ -128,8 +138,7 @@ __global__ void __launch_bounds__(TPB, 1536 / TPB) scores_kernel(zn_scores_args 
     float bar_x = -INFINITY;
     const auto read_bar = [&]() {
         bar = list.bar;
-        const uint32_t u = (uint32_t)(bar >> 32);
-        bar_x = bar == 0 ? -INFINITY : __uint_as_float((u & 0x80000000u) ? u & 0x7fffffffu : ~u);
+        bar_x = bar == 0 ? -INFINITY : key_logit(bar);
     };
     const float4 *p = reinterpret_cast<const float4 *>(x + from) + threadIdx.x;
     const float4 none = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
@@ -270,7 +279,13 @@ __global__ void __launch_bounds__(TPB, 1536 / TPB) scores_kernel(zn_scores_args 
                 return i < pieces * k ? __ldcg(reinterpret_cast<const unsigned long long *>(scratch + (r * pieces + i / k) * record + 4) + i % k) : 0ull;
             };
             bar = list.bar;
-            for (int i = threadIdx.x; i < pieces * k; i += TPB) put_key(list, key_at(i), bar);
+            for (int i0 = threadIdx.x; i0 < pieces * k; i0 += 4 * TPB) {
+                unsigned long long key[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) key[j] = key_at(i0 + j * TPB);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) put_key(list, key[j], bar);
+            }
             __syncthreads();
             if (list.count > LIST) {
                 __syncthreads();
@@ -291,11 +306,10 @@ __global__ void __launch_bounds__(TPB, 1536 / TPB) scores_kernel(zn_scores_args 
         }
         if (a.entropy) a.entropy[r] = bad ? nan : empty ? 0.f : ls - st.w * 0.6931471805599453f / st.s;
         if (a.logprob) {
-            const int64_t t = a.tokens[r];
             float lp = 0.f;
-            if (t >= a.vocab) { zn_bad_token(status); lp = nan; }
+            if (token >= a.vocab) { zn_bad_token(status); lp = nan; }
             else if (bad) lp = nan;
-            else if (t >= 0) lp = empty ? -INFINITY : (x[t] - st.m) * inv_t - ls;
+            else if (token >= 0) lp = empty ? -INFINITY : (given - st.m) * inv_t - ls;
             a.logprob[r] = lp;
         }
     }
@@ -303,7 +317,7 @@ __global__ void __launch_bounds__(TPB, 1536 / TPB) scores_kernel(zn_scores_args 
         const unsigned long long o = j < kept && !bad ? list.key[j] : 0ull;
         const int64_t col = (int64_t)(0xffffffffu - (uint32_t)o);
         a.top_tokens[r * k + j] = o ? (int32_t)col : -1;
-        a.top_logprobs[r * k + j] = bad ? nan : o ? (x[col] - st.m) * inv_t - ls : -INFINITY;
+        a.top_logprobs[r * k + j] = bad ? nan : o ? (key_logit(o) - st.m) * inv_t - ls : -INFINITY;
     }
 }
 
