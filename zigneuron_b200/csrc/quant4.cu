@@ -32,39 +32,46 @@ __device__ __forceinline__ float apply_act(int act, float x) {
     }
 }
 
-// Place of word w (codes 8 w .. 8 w + 7 of a column) in the packed row.
-__device__ __forceinline__ int64_t word_place(int64_t w) { return (w & ~15ll) + (w & 3) * 4 + ((w & 15) >> 2); }
-
-// One thread per (group, column); neighbouring threads take neighbouring columns, so the reads of w are whole lines.
-__global__ void quantize_kernel(const float *__restrict__ w, uint32_t *__restrict__ packed, float *__restrict__ scales, int64_t n, int64_t k,
-                                int64_t group) {
-    const int64_t words = (k + 127) / 128 * 16, groups = (k + group - 1) / group, padded = words * 8 / group;
-    const int64_t total = n * padded;
-    for (int64_t at = (int64_t)blockIdx.x * TPB + threadIdx.x; at < total; at += (int64_t)gridDim.x * TPB) {
-        const int64_t j = at % n, g = at / n;
-        const int64_t lo = g * group, hi = min(k, lo + group);
-        float top = 0.f;
-        bool bad = false;
-        for (int64_t i = lo; i < hi; ++i) {
-            const float v = w[i * n + j];
-            if (!(fabsf(v) < INFINITY)) bad = true;
-            top = fmaxf(top, fabsf(v));
+// A block takes 32 columns and 128 weights of each: a warp reads 16 rows of w as whole lines, the groups' largest values meet
+// in shared memory, and so do the words, which leave as 64 bytes per column.  Measured, 16,384 x 8192 in groups of
+// 128: 228 us, bound by the divisions, against 582 with one thread per group (its words went out four bytes at a time).
+constexpr int QUANT_COLUMNS = 32, QUANT_ROWS = 16;
+__global__ void __launch_bounds__(TPB) quantize_kernel(const float *__restrict__ w, uint32_t *__restrict__ packed, float *__restrict__ scales,
+                                                       int64_t n, int64_t k, int group, int64_t column_blocks) {
+    __shared__ float most[TPB / 32][QUANT_COLUMNS];
+    __shared__ __align__(16) uint32_t word[QUANT_COLUMNS][20];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int64_t block = blockIdx.x / column_blocks, first = blockIdx.x % column_blocks * QUANT_COLUMNS, j = first + lane;
+    const int64_t i0 = block * 128 + warp * QUANT_ROWS, blocks = (k + 127) / 128, groups = (k + group - 1) / group;
+    float v[QUANT_ROWS], top = 0.f;
+#pragma unroll
+    for (int i = 0; i < QUANT_ROWS; ++i) v[i] = j < n && i0 + i < k ? __ldcs(w + (i0 + i) * n + j) : 0.f;
+#pragma unroll
+    for (int i = 0; i < QUANT_ROWS; ++i) top = fabsf(v[i]) < INFINITY ? fmaxf(top, fabsf(v[i])) : INFINITY;      // NaN counts as infinity
+    most[warp][lane] = top;
+    __syncthreads();
+    const int warps = group / QUANT_ROWS, lead = warp / warps * warps;       // of this warp's group
+    for (int i = 0; i < warps; ++i) top = fmaxf(top, most[lead + i][lane]);
+    const bool bad = top == INFINITY;
+    const float scale = __fdiv_rn(top, 7.f);
+    const int64_t g = i0 / group;
+    if (warp == lead && j < n && g < groups) scales[j * groups + g] = bad ? zn_nan() : scale;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        uint32_t codes = 0;
+#pragma unroll
+        for (int b = 0; b < 8; ++b) {
+            int code = 8;
+            if (!bad && scale > 0.f) code = 8 + (int)fminf(7.f, fmaxf(-7.f, rintf(__fdiv_rn(v[8 * h + b], scale))));
+            codes |= (uint32_t)code << (4 * b);
         }
-        const float scale = __fdiv_rn(top, 7.f);
-        if (g < groups) scales[j * groups + g] = bad ? __int_as_float(0x7fffffff) : scale;
-        for (int64_t i = lo; i < lo + group; i += 8) {
-            uint32_t word = 0;
-            for (int b = 0; b < 8; ++b) {
-                int code = 8;
-                if (i + b < hi && !bad && scale > 0.f) {
-                    const float q = rintf(__fdiv_rn(w[(i + b) * n + j], scale));
-                    code = 8 + (int)fminf(7.f, fmaxf(-7.f, q));
-                }
-                word |= (uint32_t)code << (4 * b);
-            }
-            packed[j * words + word_place(i / 8)] = word;
-        }
+        const int at = 2 * warp + h;
+        word[lane][(at & 3) * 4 + (at >> 2)] = codes;
     }
+    __syncthreads();
+    const int column = threadIdx.x >> 2, part = threadIdx.x & 3;
+    if (threadIdx.x < 4 * QUANT_COLUMNS && first + column < n)
+        reinterpret_cast<uint4 *>(packed)[((first + column) * blocks + block) * 4 + part] = *reinterpret_cast<const uint4 *>(&word[column][4 * part]);
 }
 
 // x as the product reads it.  For each 32 weights and each eight columns of the tile (column 3 r + part of row r): the 16
@@ -369,16 +376,18 @@ __global__ void __launch_bounds__(WARPS * 32 + 64) matmul4_kernel(const __grid_c
 
 zn_token_plan zn_plan_quantize4(size_t n, size_t k, int sms) {
     zn_token_plan p;
+    (void)sms;
     p.threads = TPB;
-    const int64_t want = (int64_t)((n * ((k + 127) / 128) + TPB - 1) / TPB);
-    p.blocks = want < (int64_t)sms * 8 ? want : (int64_t)sms * 8;
+    p.blocks = (int64_t)((n + QUANT_COLUMNS - 1) / QUANT_COLUMNS * ((k + 127) / 128));
     return p;
 }
 
 zn_status zn_k_quantize4(zn_ctx *ctx, const float *w, uint32_t *packed, float *scales, size_t n, size_t k, size_t group) {
     const zn_token_plan p = zn_plan_quantize4(n, k, ctx->sm_count);
+    if (p.blocks > 0x7fffffff) return zn_fail(ctx, ZN_ERR_SHAPE, "quantize4: %zu x %zu weights are too many for one launch", n, k);
     zn_launch_scope scope(ctx, ZN_PROF_CONVERT, 0, 4.5 * n * k);
-    quantize_kernel<<<(unsigned)p.blocks, p.threads, 0, ctx->stream>>>(w, packed, scales, (int64_t)n, (int64_t)k, (int64_t)group);
+    quantize_kernel<<<(unsigned)p.blocks, p.threads, 0, ctx->stream>>>(w, packed, scales, (int64_t)n, (int64_t)k, (int)group,
+                                                                       (int64_t)((n + QUANT_COLUMNS - 1) / QUANT_COLUMNS));
     ZN_CUDA(ctx, cudaGetLastError());
     return ZN_OK;
 }
