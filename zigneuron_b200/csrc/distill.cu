@@ -402,9 +402,9 @@ __global__ void __launch_bounds__(THREADS + 64 + 32 * MAX_RING) distill_kernel(z
 
 // Blocks per row, values of a slice on chip, places in the ring, and threads.  A row is cut into as few slices as leave
 // room for three of them in a block, eight at most (two places in the ring: 621 instead of 457 us for 2048 rows of 131,072);
-// larger vocabularies get a shorter ring, and what does not fit even once is read a second time.  (Clusters of sixteen, which would hold twice the vocabulary in registers: 592 us for 1024 rows of
-// 200,003 against 472.)  Where there are fewer rows than SMs they are spread over more blocks, down to 2048 values
-// each.
+// larger vocabularies get a shorter ring, and what does not fit even once is read a second time.  (Clusters of sixteen,
+// which would hold twice the vocabulary in registers: 592 us for 1024 rows of 200,003 against 472.)  Where there are fewer
+// rows than SMs they are spread over more blocks, down to 2048 values each.
 constexpr size_t SMEM = 227 * 1024 - sizeof(Shared) - 64;
 struct Plan {
     int share, slice, keep, ring, threads;

@@ -166,8 +166,8 @@ __global__ void __launch_bounds__(TPB, 1536 / TPB) scores_kernel(zn_scores_args 
             float mine = top;
             for (int o = width / 2; o > 0; o /= 2) mine = fmaxf(mine, __shfl_xor_sync(0xffffffffu, mine, o));
             if (threadIdx.x % width == 0) largest[threadIdx.x / width] = mine;
-            held = list.count;                       // the values around the aligned part
             __syncthreads();
+            held = list.count;                       // the values around the aligned part
             if (threadIdx.x < groups) {
                 mine = largest[threadIdx.x];
                 int above = 0, reach = 0;
@@ -322,8 +322,7 @@ __global__ void __launch_bounds__(TPB, 1536 / TPB) scores_kernel(zn_scores_args 
 }
 
 // Gradient: every value by itself, one read and one write of the block, bound by HBM (2048 x 131,072: 350 us, 6.1 TB/s, 0.94
-// of a copy).  A block takes 4096 columns of a row, stores 16
-// bytes at a time and loads as wide where both rows stand alike.
+// of a copy).  A block takes 4096 columns of a row, stores 16 bytes at a time and loads as wide where both rows stand alike.
 constexpr int GRAD_TILE = GRAD_TPB * 16;
 __global__ void __launch_bounds__(GRAD_TPB) scores_grad_kernel(zn_scores_grad_args a, int pieces, int *status) {
     const int64_t r = blockIdx.x / pieces;
